@@ -4,7 +4,9 @@ ARCH    ?= gfx950
 CSRC    := mcmc_amd/csrc
 OUT     := mcmc_amd/lib
 OBJ     := build/obj
-HIPFLAGS := -O3 --offload-arch=$(ARCH) -fPIC -std=c++17 -Wall -Wno-unused-function -Iinclude -I$(CSRC)
+# packed fp32 VALU instructions (v_pk_add/mul/fma_f32) stay off: some of their forms have given wrong results on these devices
+NOPK    := -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS := -O3 $(NOPK) --offload-arch=$(ARCH) -fPIC -std=c++17 -Wall -Wno-unused-function -Iinclude -I$(CSRC)
 
 HIP_SRCS := $(wildcard $(CSRC)/*.hip)
 CPP_SRCS := $(wildcard $(CSRC)/*.cpp)
@@ -30,7 +32,7 @@ $(OUT)/libmcmc_hip.so: $(OBJS)
 # adds a device-less test context so that the argument validation of every entry point runs on a box without a GPU.
 # tests/abi_check.cpp drives it; tests/test_host_sanitizer.py runs `make asan` and the binary.
 ASAN_OBJ := build/asan
-ASANFLAGS := -O1 -g --offload-arch=$(ARCH) -fPIC -std=c++17 -Wall -Wno-unused-function -Iinclude -I$(CSRC) -DMCMC_DRY_CTX \
+ASANFLAGS := -O1 -g $(NOPK) --offload-arch=$(ARCH) -fPIC -std=c++17 -Wall -Wno-unused-function -Iinclude -I$(CSRC) -DMCMC_DRY_CTX \
              -Xarch_host -fsanitize=address -Xarch_host -fsanitize=undefined -Xarch_host -fno-sanitize-recover=undefined \
              -Xarch_host -fno-omit-frame-pointer
 ASAN_OBJS := $(patsubst $(CSRC)/%.hip,$(ASAN_OBJ)/%.o,$(HIP_SRCS)) $(patsubst $(CSRC)/%.cpp,$(ASAN_OBJ)/%.o,$(CPP_SRCS))
