@@ -44,6 +44,7 @@ extern "C" {
  * with masks and mcmc_forward_dropout reject it.  xpack / wpack images are per dtype: pack_x,
  * sample_weights and forward of one predict must name the same dtype. */
 #define MCMC_DT_BF16_FAST 2
+#define MCMC_DT_F16 3 /* IEEE half: mcmc_grouped_linear_* and mcmc_dropout_* only */
 
 #define MCMC_NOISE_NONE 0     /* W = mu            (sample=False, bayesian_ensemble.py:45-47) */
 #define MCMC_NOISE_INJECTED 1 /* W = mu + eps*exp(rho), eps supplied by the caller          */
@@ -423,6 +424,69 @@ int mcmc_tft_adamw(mcmc_ctx* ctx, float* P, float* PT, int num_features, const f
                    float* grad, float* adam_m, float* adam_v, double* norm_scratch, float lr, float beta1,
                    float beta2, float adam_eps, float weight_decay, float max_norm, int64_t step,
                    float* gnorm, mcmc_stream_t stream);
+
+/* ---- operators over ragged groups of rows ---------------------------------------------------- */
+/* The reference hands every member the whole batch (bayesian_ensemble.py:160-169); these serve members (or experts) that each own
+ * a different share of the rows, and layers of any width.  Limits: rows <= MCMC_GROUPED_MAX_ROWS; n_groups, n_in and n_out in
+ * [1, MCMC_GROUPED_MAX_DIM].
+ *
+ * mcmc_group_rows: the rows sorted stably by group.
+ *   ids     [rows] int32 (id_bytes 4) or int64 (8): the row's group; a value outside 0..n_groups-1 = no group
+ *   order   [rows] int32: the rows of group 0 in their order, then group 1's, ..., then the rows of no group
+ *   offsets [n_groups + 1] int32: group g is order[offsets[g]] .. order[offsets[g+1] - 1]
+ * n_groups <= MCMC_GROUP_ROWS_MAX_GROUPS.  workspace: mcmc_group_rows_workspace_bytes(rows, n_groups) bytes (0 for small
+ * batches: NULL is fine), 16-byte aligned, contents irrelevant before and after. */
+#define MCMC_GROUPED_MAX_ROWS ((int64_t)1 << 30)
+#define MCMC_GROUPED_MAX_DIM (1 << 30)
+#define MCMC_GROUP_ROWS_MAX_GROUPS 4096
+int64_t mcmc_group_rows_workspace_bytes(int64_t rows, int n_groups);
+int mcmc_group_rows(mcmc_ctx* ctx, const void* ids, int id_bytes, int64_t rows, int n_groups, int32_t* order,
+                    int32_t* offsets, void* workspace, mcmc_stream_t stream);
+
+/* y[r] = weight[g] x[r] + bias[g] for every row r of every group g (F.linear, bayesian_ensemble.py:49, with the group's own
+ * weights); rows of no group get 0.
+ *   dtype   MCMC_DT_F32, MCMC_DT_BF16 or MCMC_DT_F16: of x, weight, bias, y and all gradients; sums are fp32
+ *   x       [rows, n_in], ld_x elements between rows (any, also 0);  y [rows, n_out] dense
+ *   weight  [n_groups, n_out, n_in] dense;  bias [n_groups, n_out] or NULL
+ *   order   [rows] int32, every row once, or NULL (row r is at position r);  offsets [n_groups + 1] int32, from 0, not
+ *           decreasing, at most rows: device memory, e.g. from mcmc_group_rows.  Positions from offsets[n_groups] on are rows of
+ *           no group.  Values outside these bounds give wrong results but no access outside the arrays.
+ * Pointers need the alignment of their elements only. */
+int mcmc_grouped_linear_forward(mcmc_ctx* ctx, int dtype, const void* x, int64_t ld_x, int64_t rows, const int32_t* order,
+                                const int32_t* offsets, int n_groups, int n_in, int n_out, const void* weight,
+                                const void* bias, void* y, mcmc_stream_t stream);
+/* dx[r] = weight[g]^T dy[r]; rows of no group: 0.  dy [rows, n_out], ld_dy elements between rows; dx [rows, n_in] dense. */
+int mcmc_grouped_linear_grad_input(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, int64_t rows,
+                                   const int32_t* order, const int32_t* offsets, int n_groups, int n_in, int n_out,
+                                   const void* weight, void* dx, mcmc_stream_t stream);
+/* dweight[g] = sum of dy[r] x[r]^T over the rows of g, dbias[g] = sum of dy[r] (dbias may be NULL); groups without rows: 0.
+ * Partial sums meet in a fixed order in workspace (mcmc_grouped_linear_workspace_bytes, may be 0; 16-byte aligned): no atomics,
+ * the same bits every time. */
+int64_t mcmc_grouped_linear_workspace_bytes(int64_t rows, int n_groups, int n_in, int n_out);
+int mcmc_grouped_linear_grad_weight(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
+                                    int64_t rows, const int32_t* order, const int32_t* offsets, int n_groups, int n_in,
+                                    int n_out, void* dweight, void* dbias, void* workspace, mcmc_stream_t stream);
+
+/* ---- dropout of one layer -------------------------------------------------------------------- */
+/* y = keep ? act(x) * s : 0, s = fp32(1/(1-p_drop)) (F.elu then nn.Dropout, bayesian_ensemble.py:85-86), for rows of any width; the
+ * mask is drawn from the 'MASK' stream of mcmc_forward_dropout / mcmc_train_forward and never stored: column c of row r is element
+ * elem_begin + c of global row row_begin + r of `pair` (elem_begin 0 / 256 / 384 and pair = the global pair id: the masks of
+ * the three hidden layers of a training step).  A dropped element is 0 whatever x holds.
+ *   dtype      MCMC_DT_F32, MCMC_DT_BF16 or MCMC_DT_F16
+ *   activation MCMC_ACT_NONE or MCMC_ACT_ELU (alpha 1)
+ *   seed_dev   device uint64 read when the kernel runs (a captured hipGraph can be replayed with a new key); NULL: `seed`
+ *   0 <= p_drop < 1; elem_begin a multiple of 16, elem_begin + width <= 2^32; row_begin + rows <= 2^32; 0 <= pair < 2^32
+ * ld_*: elements between rows.  Pointers need the alignment of their elements only. */
+#define MCMC_ACT_NONE 0
+#define MCMC_ACT_ELU 1
+int mcmc_dropout_forward(mcmc_ctx* ctx, int dtype, int activation, const void* x, int64_t ld_x, int64_t rows,
+                         int64_t width, uint64_t seed, const uint64_t* seed_dev, float p_drop, int64_t pair,
+                         int64_t row_begin, int64_t elem_begin, void* y, int64_t ld_y, mcmc_stream_t stream);
+/* dx = keep ? dy * act'(x) * s : 0 with the same mask, drawn again; x: the forward's input (MCMC_ACT_NONE: not read, may be NULL). */
+int mcmc_dropout_backward(mcmc_ctx* ctx, int dtype, int activation, const void* dy, int64_t ld_dy, const void* x,
+                          int64_t ld_x, int64_t rows, int64_t width, uint64_t seed, const uint64_t* seed_dev,
+                          float p_drop, int64_t pair, int64_t row_begin, int64_t elem_begin, void* dx, int64_t ld_dx,
+                          mcmc_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -53,7 +53,7 @@ extern "C" {
 
 const char* mcmc_last_error(void) { return g_err; }
 
-int mcmc_abi_version(void) { return 21; }
+int mcmc_abi_version(void) { return 22; }
 
 int mcmc_ctx_create(int device, mcmc_ctx** out) {
     MCMC_REQUIRE(out != nullptr, "out is NULL");
@@ -711,6 +711,129 @@ int mcmc_tft_adamw(mcmc_ctx* ctx, float* P, float* PT, int num_features, const f
     MCMC_REQUIRE(beta1 >= 0.0f && beta1 < 1.0f && beta2 >= 0.0f && beta2 < 1.0f, "betas must be in [0, 1)");
     return launch_flat_update(P, mcmc_tft_param_count(num_features), dP, n_partials, grad, adam_m, adam_v, norm_scratch, lr, beta1, beta2,
                               adam_eps, weight_decay, max_norm, step, gnorm, PT, num_features, (hipStream_t)stream);
+}
+
+// ---- operators over ragged groups of rows ----
+static int check_group_rows(int64_t rows, int n_groups) {
+    MCMC_REQUIRE(rows >= 0 && rows <= MCMC_GROUPED_MAX_ROWS, "rows must be in [0, 2^30] (got %lld)", (long long)rows);
+    MCMC_REQUIRE(n_groups >= 1 && n_groups <= MCMC_GROUP_ROWS_MAX_GROUPS, "n_groups must be in [1, %d] (got %d)", MCMC_GROUP_ROWS_MAX_GROUPS, n_groups);
+    return MCMC_OK;
+}
+
+int64_t mcmc_group_rows_workspace_bytes(int64_t rows, int n_groups) {
+    if (int rc = check_group_rows(rows, n_groups)) return rc;
+    return group_rows_workspace_bytes(rows, n_groups);
+}
+
+int mcmc_group_rows(mcmc_ctx* ctx, const void* ids, int id_bytes, int64_t rows, int n_groups, int32_t* order, int32_t* offsets,
+                    void* workspace, mcmc_stream_t stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_group_rows(rows, n_groups)) return rc;
+    MCMC_REQUIRE(id_bytes == 4 || id_bytes == 8, "id_bytes must be 4 or 8 (got %d)", id_bytes);
+    MCMC_REQUIRE(offsets, "offsets is NULL");
+    MCMC_REQUIRE(rows == 0 || (ids && order), "ids / order is NULL");
+    MCMC_REQUIRE(reinterpret_cast<uintptr_t>(ids) % (unsigned)id_bytes == 0, "ids must be %d-byte aligned", id_bytes);
+    if (group_rows_workspace_bytes(rows, n_groups) > 0)
+        MCMC_REQUIRE(workspace && aligned16(workspace), "workspace must be 16-byte aligned device memory (mcmc_group_rows_workspace_bytes)");
+    return launch_group_rows(ids, id_bytes, rows, n_groups, order, offsets, workspace, (hipStream_t)stream);
+}
+
+static int check_operand_dtype(int dtype) {
+    MCMC_REQUIRE(dtype == MCMC_DT_F32 || dtype == MCMC_DT_BF16 || dtype == MCMC_DT_F16, "dtype must be MCMC_DT_F32, MCMC_DT_BF16 or MCMC_DT_F16 (got %d)",
+                 dtype);
+    return MCMC_OK;
+}
+static bool aligned_for(int dtype, const void* p) { return reinterpret_cast<uintptr_t>(p) % (dtype == MCMC_DT_F32 ? 4u : 2u) == 0; }
+
+static int check_grouped_dims(int64_t rows, int n_groups, int n_in, int n_out) {
+    MCMC_REQUIRE(rows >= 0 && rows <= MCMC_GROUPED_MAX_ROWS, "rows must be in [0, 2^30] (got %lld)", (long long)rows);
+    for (int n : {n_groups, n_in, n_out})
+        MCMC_REQUIRE(n >= 1 && n <= MCMC_GROUPED_MAX_DIM, "n_groups, n_in and n_out must be in [1, 2^30] (got %d, %d, %d)", n_groups, n_in, n_out);
+    return MCMC_OK;
+}
+
+int64_t mcmc_grouped_linear_workspace_bytes(int64_t rows, int n_groups, int n_in, int n_out) {
+    if (int rc = check_grouped_dims(rows, n_groups, n_in, n_out)) return rc;
+    return grouped_linear_workspace_bytes(rows, n_groups, n_in, n_out);
+}
+
+int mcmc_grouped_linear_forward(mcmc_ctx* ctx, int dtype, const void* x, int64_t ld_x, int64_t rows, const int32_t* order, const int32_t* offsets,
+                                int n_groups, int n_in, int n_out, const void* weight, const void* bias, void* y, mcmc_stream_t stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_operand_dtype(dtype)) return rc;
+    if (int rc = check_grouped_dims(rows, n_groups, n_in, n_out)) return rc;
+    MCMC_REQUIRE(ld_x >= 0, "ld_x < 0");
+    if (rows == 0) return MCMC_OK;
+    MCMC_REQUIRE(x && offsets && weight && y, "x / offsets / weight / y is NULL");
+    MCMC_REQUIRE(aligned_for(dtype, x) && aligned_for(dtype, weight) && aligned_for(dtype, bias) && aligned_for(dtype, y),
+                 "x, weight, bias and y must be aligned to their elements");
+    return launch_grouped_linear_forward(dtype, x, ld_x, rows, order, offsets, n_groups, n_in, n_out, weight, bias, y, (hipStream_t)stream);
+}
+
+int mcmc_grouped_linear_grad_input(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, int64_t rows, const int32_t* order,
+                                   const int32_t* offsets, int n_groups, int n_in, int n_out, const void* weight, void* dx, mcmc_stream_t stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_operand_dtype(dtype)) return rc;
+    if (int rc = check_grouped_dims(rows, n_groups, n_in, n_out)) return rc;
+    MCMC_REQUIRE(ld_dy >= 0, "ld_dy < 0");
+    if (rows == 0) return MCMC_OK;
+    MCMC_REQUIRE(dy && offsets && weight && dx, "dy / offsets / weight / dx is NULL");
+    MCMC_REQUIRE(aligned_for(dtype, dy) && aligned_for(dtype, weight) && aligned_for(dtype, dx), "dy, weight and dx must be aligned to their elements");
+    return launch_grouped_linear_grad_input(dtype, dy, ld_dy, rows, order, offsets, n_groups, n_in, n_out, weight, dx, (hipStream_t)stream);
+}
+
+int mcmc_grouped_linear_grad_weight(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows,
+                                    const int32_t* order, const int32_t* offsets, int n_groups, int n_in, int n_out, void* dweight,
+                                    void* dbias, void* workspace, mcmc_stream_t stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_operand_dtype(dtype)) return rc;
+    if (int rc = check_grouped_dims(rows, n_groups, n_in, n_out)) return rc;
+    MCMC_REQUIRE(ld_dy >= 0 && ld_x >= 0, "ld_dy / ld_x < 0");
+    MCMC_REQUIRE(offsets && dweight, "offsets / dweight is NULL");
+    MCMC_REQUIRE(rows == 0 || (dy && x), "dy / x is NULL");
+    MCMC_REQUIRE(aligned_for(dtype, dy) && aligned_for(dtype, x) && aligned_for(dtype, dweight) && aligned_for(dtype, dbias),
+                 "dy, x, dweight and dbias must be aligned to their elements");
+    if (grouped_linear_workspace_bytes(rows, n_groups, n_in, n_out) > 0)
+        MCMC_REQUIRE(workspace && aligned16(workspace), "workspace must be 16-byte aligned device memory (mcmc_grouped_linear_workspace_bytes)");
+    return launch_grouped_linear_grad_weight(dtype, dy, ld_dy, x, ld_x, rows, order, offsets, n_groups, n_in, n_out, dweight, dbias, workspace,
+                                             (hipStream_t)stream);
+}
+
+// ---- dropout of one layer ----
+static int dropout_impl(mcmc_ctx* ctx, int dtype, int activation, bool backward, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
+                        int64_t rows, int64_t width, uint64_t seed, const uint64_t* seed_dev, float p_drop, int64_t pair, int64_t row_begin,
+                        int64_t elem_begin, void* out, int64_t ld_out, mcmc_stream_t stream) {
+    constexpr int64_t k32 = (int64_t)1 << 32;
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_operand_dtype(dtype)) return rc;
+    MCMC_REQUIRE(activation == MCMC_ACT_NONE || activation == MCMC_ACT_ELU, "activation must be MCMC_ACT_NONE or MCMC_ACT_ELU (got %d)", activation);
+    MCMC_REQUIRE(rows >= 0 && width >= 0 && width < k32 / 2, "rows must be >= 0 and width in [0, 2^31-1] (got %lld, %lld)", (long long)rows, (long long)width);
+    MCMC_REQUIRE(p_drop >= 0.0f && p_drop < 1.0f, "p_drop must be in [0, 1)");
+    MCMC_REQUIRE(pair >= 0 && pair < k32, "pair must be in [0, 2^32) (got %lld)", (long long)pair);
+    MCMC_REQUIRE(row_begin >= 0 && row_begin <= k32 && rows <= k32 - row_begin, "row_begin + rows must be in [0, 2^32]");
+    MCMC_REQUIRE(elem_begin >= 0 && elem_begin % 16 == 0 && elem_begin <= k32 - width, "elem_begin must be a multiple of 16, elem_begin + width in [0, 2^32]");
+    MCMC_REQUIRE(ld_x >= 0 && ld_dy >= 0, "ld < 0");
+    MCMC_REQUIRE(rows <= 1 || ld_out >= width, "rows of the result overlap (ld %lld, width %lld)", (long long)ld_out, (long long)width);
+    if (rows == 0 || width == 0) return MCMC_OK;
+    MCMC_REQUIRE(out && (backward ? dy && (x || activation == MCMC_ACT_NONE) : x != nullptr), "x / dy / result is NULL");
+    MCMC_REQUIRE(aligned_for(dtype, x) && aligned_for(dtype, dy) && aligned_for(dtype, out), "x, dy and the result must be aligned to their elements");
+    MCMC_REQUIRE((reinterpret_cast<uintptr_t>(seed_dev) & 7u) == 0, "seed_dev must be 8-byte aligned");
+    return launch_dropout(dtype, activation == MCMC_ACT_ELU, backward, x, ld_x, dy, ld_dy, rows, width, seed, seed_dev, p_drop, (uint32_t)pair,
+                          (uint32_t)row_begin, (uint32_t)elem_begin, out, ld_out, (hipStream_t)stream);
+}
+
+int mcmc_dropout_forward(mcmc_ctx* ctx, int dtype, int activation, const void* x, int64_t ld_x, int64_t rows, int64_t width, uint64_t seed,
+                         const uint64_t* seed_dev, float p_drop, int64_t pair, int64_t row_begin, int64_t elem_begin, void* y, int64_t ld_y,
+                         mcmc_stream_t stream) {
+    return dropout_impl(ctx, dtype, activation, false, nullptr, 0, x, ld_x, rows, width, seed, seed_dev, p_drop, pair, row_begin, elem_begin, y,
+                        ld_y, stream);
+}
+
+int mcmc_dropout_backward(mcmc_ctx* ctx, int dtype, int activation, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows,
+                          int64_t width, uint64_t seed, const uint64_t* seed_dev, float p_drop, int64_t pair, int64_t row_begin,
+                          int64_t elem_begin, void* dx, int64_t ld_dx, mcmc_stream_t stream) {
+    return dropout_impl(ctx, dtype, activation, true, dy, ld_dy, x, ld_x, rows, width, seed, seed_dev, p_drop, pair, row_begin, elem_begin, dx,
+                        ld_dx, stream);
 }
 
 }  // extern "C"

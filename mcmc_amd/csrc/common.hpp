@@ -150,4 +150,19 @@ int launch_flat_update(float* param, int64_t n, const float* dP, int B, float* g
                        float beta1, float beta2, float adam_eps, float weight_decay, float max_norm, int64_t step, float* gnorm,
                        float* PT, int F, hipStream_t s);
 
+// operators over ragged groups of rows, and the dropout of one layer
+int64_t group_rows_workspace_bytes(int64_t rows, int G);
+int launch_group_rows(const void* ids, int id_bytes, int64_t rows, int G, int* order, int* offsets, void* ws, hipStream_t s);
+int launch_grouped_linear_forward(int dtype, const void* x, int64_t ld_x, int64_t rows, const int* order, const int* offsets, int G, int n_in,
+                                  int n_out, const void* weight, const void* bias, void* y, hipStream_t s);
+int launch_grouped_linear_grad_input(int dtype, const void* dy, int64_t ld_dy, int64_t rows, const int* order, const int* offsets, int G, int n_in,
+                                     int n_out, const void* weight, void* dx, hipStream_t s);
+int64_t grouped_linear_workspace_bytes(int64_t rows, int G, int n_in, int n_out);
+int launch_grouped_linear_grad_weight(int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows, const int* order,
+                                      const int* offsets, int G, int n_in, int n_out, void* dweight, void* dbias, void* ws, hipStream_t s);
+// backward: out = dx from dy (and x, the forward's input, with an activation)
+int launch_dropout(int dtype, bool elu, bool backward, const void* x, int64_t ld_x, const void* dy, int64_t ld_dy, int64_t rows, int64_t width,
+                   uint64_t seed, const uint64_t* seed_dev, float p_drop, uint32_t pair, uint32_t row_begin, uint32_t elem_begin, void* out,
+                   int64_t ld_out, hipStream_t s);
+
 }  // namespace mcmc

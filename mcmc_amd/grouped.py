@@ -1,0 +1,242 @@
+"""Layers whose rows belong to groups: one member (or expert) per group, each with its own share of the rows.
+
+The reference hands every member the whole batch (bayesian_ensemble.py:160-169).  Here the rows are routed first and a layer's
+product runs over the ragged groups in one launch:
+
+    groups = group_rows(ids, n_members)                       # ids[r] = the member of row r
+    h = x
+    for i, (w, b) in enumerate(hidden):                       # w [members, out, in], b [members, out]
+        h = philox_dropout(grouped_linear(h, w, groups, b), 0.1, seed, activation="elu", elem_begin=elem[i])
+    y = grouped_linear(h, w_out, groups, b_out)
+
+All arithmetic is in libmcmc_hip.so (``mcmc_group_rows``, ``mcmc_grouped_linear_*``, ``mcmc_dropout_*``); gradients are ordinary
+autograd.  There is no CPU path.  Every call runs on the current stream of its tensors' device and allocates what it needs from
+torch, nothing is kept from one call for the next, so calls may be captured into HIP graphs.
+"""
+from __future__ import annotations
+
+import math
+from contextlib import nullcontext
+from typing import NamedTuple, Optional, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .engine import Engine, _p, _require_gpu, _stream
+
+_DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+_ACT = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "elu": _lib.ACT_ELU}
+_U64 = 0xFFFFFFFFFFFFFFFF
+_MAX_GROUPS = 4096       # MCMC_GROUP_ROWS_MAX_GROUPS
+_MAX_DIM = 1 << 30       # MCMC_GROUPED_MAX_ROWS, MCMC_GROUPED_MAX_DIM
+_ENGINES = {}
+
+
+def _engine(t: torch.Tensor, what: str, **others: Optional[torch.Tensor]) -> Engine:
+    """The engine of t's device; every other tensor has to live there too."""
+    dev = _require_gpu(t, what)
+    for name, o in others.items():
+        if o is not None and _require_gpu(o, name) != dev:
+            raise ValueError(f"{name} lives on {o.device}, {what} on {t.device}")
+    eng = _ENGINES.get(dev)
+    if eng is None:
+        eng = _ENGINES[dev] = Engine(torch.device("cuda", dev))
+    return eng
+
+
+def _on(eng: Engine):
+    return nullcontext() if torch.cuda.current_device() == eng.device.index else torch.cuda.device(eng.device)
+
+
+def _dtype(t: torch.Tensor, what: str) -> int:
+    try:
+        return _DT[t.dtype]
+    except KeyError:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}") from None
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A 2-D tensor whose rows are contiguous; the distance between rows is free (views and expanded rows are read in place)."""
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """[..., width] as [rows, width] (empty tensors included)."""
+    return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+
+
+class RowGroups(NamedTuple):
+    """Which rows belong to which group.  Group g owns the rows ``order[offsets[g]:offsets[g + 1]]``; what ``order`` lists from
+    ``offsets[-1]`` on belongs to no group.
+
+    order: int32 [rows], every row once, or None where the rows lie group after group already.
+    offsets: int32 [n_groups + 1], from 0, not decreasing, at most rows."""
+    order: Optional[torch.Tensor]
+    offsets: torch.Tensor
+
+    @property
+    def n_groups(self) -> int:
+        return self.offsets.shape[0] - 1
+
+
+def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
+    """Sort the rows stably by group: ``ids`` [rows] (int32 or int64) names each row's group; an id outside 0..n_groups-1 puts the
+    row into no group (``grouped_linear`` gives it zeros).  At most 4,096 groups."""
+    if ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids must be a 1-D int32 or int64 tensor, got {ids.dtype} {tuple(ids.shape)}")
+    n_groups, rows = int(n_groups), ids.shape[0]
+    if not 1 <= n_groups <= _MAX_GROUPS:
+        raise ValueError(f"n_groups must be in [1, {_MAX_GROUPS}], got {n_groups}")
+    eng = _engine(ids, "ids")
+    with _on(eng):
+        ids = ids.contiguous()
+        ws_bytes = _lib.check(eng.lib.mcmc_group_rows_workspace_bytes(rows, n_groups), "mcmc_group_rows_workspace_bytes")
+        order = torch.empty(rows, dtype=torch.int32, device=ids.device)
+        offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=ids.device)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=ids.device) if ws_bytes else None
+        _lib.check(eng.lib.mcmc_group_rows(eng.ctx.handle, _p(ids), ids.element_size(), rows, n_groups, _p(order), _p(offsets), _p(ws), _stream()),
+                   "mcmc_group_rows")
+    return RowGroups(order, offsets)
+
+
+# ---- grouped_linear ---------------------------------------------------------------------------------------------------------
+def _forward(eng: Engine, x, weight, bias, order, offsets):
+    G, N, K = weight.shape
+    y = torch.empty(x.shape[0], N, dtype=x.dtype, device=x.device)
+    _lib.check(eng.lib.mcmc_grouped_linear_forward(eng.ctx.handle, _DT[x.dtype], _p(x), x.stride(0), x.shape[0], _p(order), _p(offsets), G, K, N,
+                                                   _p(weight), _p(bias), _p(y), _stream()), "mcmc_grouped_linear_forward")
+    return y
+
+
+def _grad_input(eng: Engine, dy, weight, order, offsets):
+    G, N, K = weight.shape
+    dx = torch.empty(dy.shape[0], K, dtype=dy.dtype, device=dy.device)
+    _lib.check(eng.lib.mcmc_grouped_linear_grad_input(eng.ctx.handle, _DT[dy.dtype], _p(dy), dy.stride(0), dy.shape[0], _p(order), _p(offsets), G, K, N,
+                                                      _p(weight), _p(dx), _stream()), "mcmc_grouped_linear_grad_input")
+    return dx
+
+
+def _grad_weight(eng: Engine, dy, x, order, offsets, G: int, want_bias: bool):
+    R, N, K = x.shape[0], dy.shape[1], x.shape[1]
+    ws_bytes = _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    dw = torch.empty(G, N, K, dtype=x.dtype, device=x.device)
+    db = torch.empty(G, N, dtype=x.dtype, device=x.device) if want_bias else None
+    _lib.check(eng.lib.mcmc_grouped_linear_grad_weight(eng.ctx.handle, _DT[x.dtype], _p(dy), dy.stride(0), _p(x), x.stride(0), R, _p(order), _p(offsets),
+                                                       G, K, N, _p(dw), _p(db), _p(ws), _stream()), "mcmc_grouped_linear_grad_weight")
+    return dw, db
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, order, offsets):
+        eng = _engine(x, "x", weight=weight, bias=bias, order=order, offsets=offsets)
+        with _on(eng):
+            x, weight = _rows(x), weight.contiguous()
+            y = _forward(eng, x, weight, None if bias is None else bias.contiguous(), order, offsets)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        ctx.eng, ctx.shape = eng, weight.shape
+        # what each gradient reads: dx the weights, dW the inputs
+        ctx.save_for_backward(x if need_w or need_b else None, weight if need_x else None, order, offsets)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        eng = ctx.eng
+        x, weight, order, offsets = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        with _on(eng):
+            dy = _rows(dy)
+            if need_x:
+                dx = _grad_input(eng, dy, weight, order, offsets)
+            if need_w or need_b:
+                dw, db = _grad_weight(eng, dy, x, order, offsets, ctx.shape[0], need_b)
+        return dx, dw if need_w else None, db, None, None
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One linear layer per group: ``y[r] = weight[g] @ x[r] + bias[g]`` with g the group of row r; rows of no group are 0.
+
+    x [rows, in]; weight [n_groups, out, in]; bias [n_groups, out]; all of one type (float32, bfloat16 or float16; sums are
+    kept in 32 bits and rounded once).  Differentiable in x, weight and bias; a group without rows gets zero gradients."""
+    order, offsets = groups
+    if x.dim() != 2 or weight.dim() != 3 or (bias is not None and bias.dim() != 2):
+        raise ValueError(f"x must be [rows, in], weight [groups, out, in], bias [groups, out]; got {tuple(x.shape)}, {tuple(weight.shape)}"
+                         + ("" if bias is None else f", {tuple(bias.shape)}"))
+    _dtype(x, "x")
+    G, N, K = weight.shape
+    if min(G, N, K) < 1 or max(G, N, K, x.shape[0]) > _MAX_DIM:
+        raise ValueError(f"every size of weight must be in [1, 2^30] and rows at most 2^30, got {tuple(weight.shape)} and {x.shape[0]} rows")
+    if x.shape[1] != K:
+        raise ValueError(f"Expected {K} input features, got {x.shape[1]}")
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise ValueError(f"x, weight and bias must have one type, got {x.dtype}, {weight.dtype}" + ("" if bias is None else f", {bias.dtype}"))
+    if bias is not None and tuple(bias.shape) != (G, N):
+        raise ValueError(f"bias must be {(G, N)}, got {tuple(bias.shape)}")
+    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (G + 1,) or not offsets.is_contiguous():
+        raise ValueError(f"groups.offsets must be a contiguous int32 [{G + 1}] tensor (n_groups + 1), got {offsets.dtype} {tuple(offsets.shape)}")
+    if order is not None and (order.dtype != torch.int32 or tuple(order.shape) != (x.shape[0],) or not order.is_contiguous()):
+        raise ValueError(f"groups.order must be None or a contiguous int32 [{x.shape[0]}] tensor (rows), got {order.dtype} {tuple(order.shape)}")
+    return _GroupedLinear.apply(x, weight, bias, order, offsets)
+
+
+# ---- philox_dropout ---------------------------------------------------------------------------------------------------------
+class _PhiloxDropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, seed_dev, act, pair, row_begin, elem_begin):
+        eng = _engine(x, "x", seed=seed_dev)
+        dt = _DT[x.dtype]
+        with _on(eng):
+            x2 = _rows(_flat(x))
+            y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+            _lib.check(eng.lib.mcmc_dropout_forward(eng.ctx.handle, dt, act, _p(x2), x2.stride(0), x2.shape[0], x2.shape[1], seed, _p(seed_dev), p, pair,
+                                                    row_begin, elem_begin, _p(y), x2.shape[1], _stream()), "mcmc_dropout_forward")
+        if ctx.needs_input_grad[0]:
+            ctx.eng, ctx.args, ctx.shape = eng, (p, seed, act, pair, row_begin, elem_begin), x.shape
+            ctx.save_for_backward(x2 if act != _lib.ACT_NONE else None, seed_dev)
+        return y.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        eng, (p, seed, act, pair, row_begin, elem_begin) = ctx.eng, ctx.args
+        x2, seed_dev = ctx.saved_tensors
+        with _on(eng):
+            dy2 = _rows(_flat(dy))
+            dx = torch.empty(dy2.shape, dtype=dy.dtype, device=dy.device)
+            _lib.check(eng.lib.mcmc_dropout_backward(eng.ctx.handle, _DT[dy.dtype], act, _p(dy2), dy2.stride(0), _p(x2), 0 if x2 is None else x2.stride(0),
+                                                     dy2.shape[0], dy2.shape[1], seed, _p(seed_dev), p, pair, row_begin, elem_begin, _p(dx), dy2.shape[1],
+                                                     _stream()), "mcmc_dropout_backward")
+        return dx.view(ctx.shape), None, None, None, None, None, None, None
+
+
+def philox_dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], *, activation: Optional[str] = None, pair: int = 0,
+                   row_begin: int = 0, elem_begin: int = 0) -> torch.Tensor:
+    """``act(x) * keep / (1 - p)`` with the mask drawn from the framework's counter-based stream where it is used, forward and
+    backward, and never stored.
+
+    The last dimension of x holds a row's elements, the others count rows (row-major).  Column c of row r is element
+    ``elem_begin + c`` of row ``row_begin + r`` of ``pair``: a batch cut into pieces draws the same masks as the whole with
+    ``row_begin`` set, and elem_begin 0 / 256 / 384 with a pair's global id gives the masks of ``mcmc_train_forward``'s three
+    hidden layers.  A dropped element is 0 whatever x holds there.
+
+    activation: None or "elu" (alpha 1), applied before the dropout.  p in [0, 1); the keep probability is (1 - p) rounded down
+    to a multiple of 2^-16.  seed: a 64-bit integer, or a one-element int64 tensor on x's device that is read when the kernel
+    runs, so that a captured graph can be replayed with other masks (keep its value until the backward pass has run)."""
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    _dtype(x, "x")
+    if activation not in _ACT:
+        raise ValueError(f"activation must be None or 'elu', got {activation!r}")
+    for name, v in (("pair", pair), ("row_begin", row_begin), ("elem_begin", elem_begin)):
+        if not 0 <= int(v) <= 1 << 32:
+            raise ValueError(f"{name} must be in [0, 2^32), got {v}")
+    seed_dev = None
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ValueError(f"a seed tensor must hold one int64, got {seed.dtype} {tuple(seed.shape)}")
+        seed, seed_dev = 0, seed
+    return _PhiloxDropout.apply(x, float(p), int(seed) & _U64, seed_dev, _ACT[activation], int(pair), int(row_begin), int(elem_begin))

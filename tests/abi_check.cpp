@@ -322,6 +322,85 @@ int main() {
     EXPECT_EINVAL(mcmc_tft_adamw(c, f, f, 0, f, 1, f, f, f, d, 1e-3f, 0.9f, 0.999f, 1e-8f, 0.01f, 1.0f, 1, nullptr, s));
     EXPECT_EINVAL(mcmc_tft_adamw(c, f, f, 11, f, 1, f, f, f, d, 1e-3f, -0.1f, 0.999f, 1e-8f, 0.01f, 1.0f, 1, nullptr, s));
 
+    // ---- ragged groups of rows, dropout of one layer ----
+    {
+        const int64_t big = ((int64_t)1 << 30) + 1, k32 = (int64_t)1 << 32;
+        for (int64_t rows : {(int64_t)-1, (int64_t)0, (int64_t)1, (int64_t)8192, (int64_t)8193, (int64_t)3650000, big - 1, big})
+            for (int groups : {-1, 0, 1, 5, 1023, 1024, 4096, 4097}) {
+                const bool ok = rows >= 0 && rows < big && groups >= 1 && groups <= MCMC_GROUP_ROWS_MAX_GROUPS;
+                const int64_t w = mcmc_group_rows_workspace_bytes(rows, groups);
+                EXPECT(w >= 0, ok);
+                if (ok && rows > 8192) EXPECT(w >= (int64_t)4 * (groups + 1), 1);
+                const bool okl = rows >= 0 && rows < big && groups >= 1;
+                for (int n : {0, 1, 64, 4096}) EXPECT(mcmc_grouped_linear_workspace_bytes(rows, groups, n, 64) >= 0, okl && n >= 1);
+            }
+        EXPECT_EINVAL(mcmc_grouped_linear_workspace_bytes(4, 1, (1 << 30) + 1, 1));
+        EXPECT(mcmc_group_rows(z, i32, 4, 4, 2, i32, i32, nullptr, s), MCMC_ESTATE);
+        EXPECT(mcmc_grouped_linear_forward(z, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, f, s), MCMC_ESTATE);
+        EXPECT(mcmc_grouped_linear_grad_input(z, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, s), MCMC_ESTATE);
+        EXPECT(mcmc_grouped_linear_grad_weight(z, 0, f, 4, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s), MCMC_ESTATE);
+        EXPECT(mcmc_dropout_forward(z, 0, 0, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s), MCMC_ESTATE);
+        EXPECT(mcmc_dropout_backward(z, 0, 0, f, 4, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s), MCMC_ESTATE);
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 2, 4, 2, i32, i32, nullptr, s));           // id_bytes
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, -1, 2, i32, i32, nullptr, s));
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, big, 2, i32, i32, v, s));
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, 4, 0, i32, i32, nullptr, s));
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, 4, 4097, i32, i32, nullptr, s));
+        EXPECT_EINVAL(mcmc_group_rows(c, nullptr, 4, 4, 2, i32, i32, nullptr, s));
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, 4, 2, nullptr, i32, nullptr, s));
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, 0, 2, i32, nullptr, nullptr, s));
+        EXPECT_EINVAL(mcmc_group_rows(c, f_odd, 8, 4, 2, i32, i32, nullptr, s));         // 8-byte ids, 4-byte aligned
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, 100000, 2, i32, i32, nullptr, s));      // workspace
+        EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, 100000, 2, i32, i32, f_odd, s));
+        for (int dt : {-1, MCMC_DT_BF16_FAST, 4}) {
+            EXPECT_EINVAL(mcmc_grouped_linear_forward(c, dt, f, 4, 4, i32, i32, 2, 4, 4, f, f, f, s));
+            EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, dt, f, 4, 4, i32, i32, 2, 4, 4, f, f, s));
+            EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, dt, f, 4, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s));
+            EXPECT_EINVAL(mcmc_dropout_forward(c, dt, 0, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
+            EXPECT_EINVAL(mcmc_dropout_backward(c, dt, 0, f, 4, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
+        }
+        EXPECT(mcmc_grouped_linear_forward(c, 0, nullptr, 4, 0, nullptr, nullptr, 2, 4, 4, nullptr, nullptr, nullptr, s), MCMC_OK);
+        EXPECT(mcmc_grouped_linear_grad_input(c, 1, nullptr, 4, 0, nullptr, nullptr, 2, 4, 4, nullptr, nullptr, s), MCMC_OK);
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, -1, 4, i32, i32, 2, 4, 4, f, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, big, i32, i32, 2, 4, 4, f, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 0, 4, 4, f, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 0, 4, f, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, nullptr, 2, 4, 4, f, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, nullptr, 4, 4, i32, i32, 2, 4, 4, f, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, nullptr, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 1, u8_odd, 4, 4, i32, i32, 2, 4, 4, f, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, -4, 4, i32, i32, 2, 4, 4, f, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, 4, 4, i32, i32, 2, 4, 4, f, u8_odd, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 4, f, -4, 4, i32, i32, 2, 4, 4, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 4, f, 4, 0, i32, nullptr, 2, 4, 4, f, f, v, s));  // dweight is written for 0 rows too
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 4, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, nullptr, 4, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s));
+        EXPECT(mcmc_grouped_linear_workspace_bytes(1000000, 2, 64, 64) > 0, 1);
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 64, f, 64, 1000000, i32, i32, 2, 64, 64, f, f, nullptr, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 64, f, 64, 1000000, i32, i32, 2, 64, 64, f, f, f_odd, s));
+        EXPECT(mcmc_dropout_forward(c, 0, 1, nullptr, 4, 0, 4, 1, nullptr, 0.1f, 0, 0, 0, nullptr, 4, s), MCMC_OK);
+        EXPECT(mcmc_dropout_backward(c, 0, 1, nullptr, 4, nullptr, 4, 4, 0, 1, nullptr, 0.1f, 0, 0, 0, nullptr, 4, s), MCMC_OK);
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 2, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));            // activation
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 4, 1, nullptr, 1.0f, 0, 0, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 4, 1, nullptr, -0.1f, 0, 0, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 4, 1, nullptr, 0.1f, k32, 0, 0, f, 4, s));          // pair
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 4, 1, nullptr, 0.1f, 0, k32 - 3, 0, f, 4, s));      // row_begin + rows
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 4, 1, nullptr, 0.1f, 0, -1, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 8, f, 4, s));            // elem_begin
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 32, 1, nullptr, 0.1f, 0, 0, k32 - 16, f, 32, s));
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, -1, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, INT64_MAX, 4, 1, nullptr, 0.1f, 0, 1, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 3, s));            // result rows overlap
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, nullptr, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, u8_odd, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_forward(c, 0, 0, f, 4, 4, 4, 1, reinterpret_cast<uint64_t*>(f_odd), 0.1f, 0, 0, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_backward(c, 0, 1, f, 4, nullptr, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));   // ELU needs x
+        EXPECT_EINVAL(mcmc_dropout_backward(c, 0, 0, nullptr, 4, nullptr, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
+        EXPECT_EINVAL(mcmc_dropout_backward(c, 0, 0, f, -4, nullptr, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
+    }
+
     // an error text longer than the thread-local buffer must be truncated, not overrun (exercised through the longest message)
     EXPECT_EINVAL(mcmc_train_backward_saved(c, f, (int64_t)1 << 40, 11, 1, 1, f, f, 0, nullptr, nullptr, nullptr, 0, 0.1f, f, 7, f, f, s));
     EXPECT(strlen(mcmc_last_error()) < 512, 1);
