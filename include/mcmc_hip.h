@@ -462,7 +462,7 @@ int mcmc_grouped_linear_grad_input(mcmc_ctx* ctx, int dtype, const void* dy, int
 /* dweight[g] = sum of dy[r] x[r]^T over the rows of g, dbias[g] = sum of dy[r] (dbias may be NULL); groups without rows: 0.
  * Partial sums meet in a fixed order in workspace (mcmc_grouped_linear_workspace_bytes, may be 0; 16-byte aligned): no atomics,
  * the same bits every time. */
-int64_t mcmc_grouped_linear_workspace_bytes(int64_t rows, int n_groups, int n_in, int n_out);
+int64_t mcmc_grouped_linear_workspace_bytes(int dtype, int64_t rows, int n_groups, int n_in, int n_out);
 int mcmc_grouped_linear_grad_weight(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
                                     int64_t rows, const int32_t* order, const int32_t* offsets, int n_groups, int n_in,
                                     int n_out, void* dweight, void* dbias, void* workspace, mcmc_stream_t stream);

@@ -119,7 +119,7 @@ SIGNATURES = {
     "mcmc_group_rows": (_i32, [_ctx_p, _ptr, _i32, _i64, _i32, _ptr, _ptr, _ptr, _stream]),
     "mcmc_grouped_linear_forward": (_i32, [_ctx_p, _i32, _ptr, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _ptr, _ptr, _ptr, _stream]),
     "mcmc_grouped_linear_grad_input": (_i32, [_ctx_p, _i32, _ptr, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _ptr, _ptr, _stream]),
-    "mcmc_grouped_linear_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32]),
+    "mcmc_grouped_linear_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32]),
     "mcmc_grouped_linear_grad_weight": (_i32, [_ctx_p, _i32, _ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _ptr, _ptr, _ptr, _stream]),
     "mcmc_dropout_forward": (_i32, [_ctx_p, _i32, _i32, _ptr, _i64, _i64, _i64, _u64, _ptr, _f32, _i64, _i64, _i64, _ptr, _i64, _stream]),
     "mcmc_dropout_backward": (_i32, [_ctx_p, _i32, _i32, _ptr, _i64, _ptr, _i64, _i64, _i64, _u64, _ptr, _f32, _i64, _i64, _i64, _ptr, _i64, _stream]),

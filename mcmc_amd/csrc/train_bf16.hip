@@ -30,6 +30,7 @@
 // History, phase timings and what bounds the kernels now: profiles/EXPERIMENTS.md section 4b.
 #include "common.hpp"
 #include "dropmask.hpp"
+#include "lds_dma.hpp"
 
 namespace mcmc {
 
@@ -184,13 +185,6 @@ __device__ __forceinline__ W0Frag load_w0(const float* __restrict__ w, int F, in
     return f;
 }
 
-// Workgroup barrier that leaves VMEM in flight: __syncthreads() drains vmcnt while an LDS-DMA load is outstanding
-// (cdna_hip_programming.md, 'Pipelining across barriers'); LDS traffic is retired by the lgkmcnt wait.
-__device__ __forceinline__ void barrier_lds_only() {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
 template <bool RAW>
 __device__ __forceinline__ void tile_barrier() {
     if (RAW) barrier_lds_only();
@@ -368,19 +362,6 @@ __device__ __forceinline__ void input_grad_store(const f32x16& acc, __bf16* hin,
 
 // SAVED: the forward kernel left the tiles in `act`; otherwise each tile's forward pass is recomputed here (two builds, so that
 // neither carries the other's registers: 128 per lane at four waves per SIMD)
-typedef __attribute__((address_space(3))) char lds_char;
-// One LDS-DMA load (global_load_lds_dwordx4: lane i's 16 bytes land at the wave-uniform LDS byte address lds_dst + 16 i), as an
-// asm statement so that hipcc does not count it: with the builtin every LDS read that follows waits vmcnt(0) for it (the
-// compiler cannot tell that the read does not alias the destination), which would expose the load in the very next phase.
-// Completion is counted by hand: s_waitcnt vmcnt(0) in the issuing wave, then a barrier, then the reads
-// (cdna_hip_programming.md, inline-asm rules: M0 is written in the statement that uses it and restored).
-__device__ __forceinline__ void glds16(const void* gsrc, unsigned lds_dst) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(gsrc), "s"(lds_dst)
-                 : "memory");
-}
 // 1-KiB pieces [p0, p1) of a saved tile, global -> LDS without registers (the saved image is the LDS image byte for byte),
 // pieces dealt round-robin to the waves
 __device__ __forceinline__ void dma_pieces(const uint4* src_tile, __bf16* lds_tile, int wave, int p0, int p1) {

@@ -119,7 +119,7 @@ def _grad_input(eng: Engine, dy, weight, order, offsets):
 
 def _grad_weight(eng: Engine, dy, x, order, offsets, G: int, want_bias: bool):
     R, N, K = x.shape[0], dy.shape[1], x.shape[1]
-    ws_bytes = _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
+    ws_bytes = _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(_DT[x.dtype], R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
     dw = torch.empty(G, N, K, dtype=x.dtype, device=x.device)
     db = torch.empty(G, N, dtype=x.dtype, device=x.device) if want_bias else None

@@ -332,9 +332,9 @@ int main() {
                 EXPECT(w >= 0, ok);
                 if (ok && rows > 8192) EXPECT(w >= (int64_t)4 * (groups + 1), 1);
                 const bool okl = rows >= 0 && rows < big && groups >= 1;
-                for (int n : {0, 1, 64, 4096}) EXPECT(mcmc_grouped_linear_workspace_bytes(rows, groups, n, 64) >= 0, okl && n >= 1);
+                for (int n : {0, 1, 64, 4096}) EXPECT(mcmc_grouped_linear_workspace_bytes(MCMC_DT_F16, rows, groups, n, 64) >= 0, okl && n >= 1);
             }
-        EXPECT_EINVAL(mcmc_grouped_linear_workspace_bytes(4, 1, (1 << 30) + 1, 1));
+        EXPECT_EINVAL(mcmc_grouped_linear_workspace_bytes(0, 4, 1, (1 << 30) + 1, 1));
         EXPECT(mcmc_group_rows(z, i32, 4, 4, 2, i32, i32, nullptr, s), MCMC_ESTATE);
         EXPECT(mcmc_grouped_linear_forward(z, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, f, s), MCMC_ESTATE);
         EXPECT(mcmc_grouped_linear_grad_input(z, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, s), MCMC_ESTATE);
@@ -377,7 +377,7 @@ int main() {
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 4, f, 4, 0, i32, nullptr, 2, 4, 4, f, f, v, s));  // dweight is written for 0 rows too
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 4, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, v, s));
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, nullptr, 4, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s));
-        EXPECT(mcmc_grouped_linear_workspace_bytes(1000000, 2, 64, 64) > 0, 1);
+        EXPECT(mcmc_grouped_linear_workspace_bytes(1, 1000000, 2, 64, 64) > 0, 1);
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 64, f, 64, 1000000, i32, i32, 2, 64, 64, f, f, nullptr, s));
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 64, f, 64, 1000000, i32, i32, 2, 64, 64, f, f, f_odd, s));
         EXPECT(mcmc_dropout_forward(c, 0, 1, nullptr, 4, 0, 4, 1, nullptr, 0.1f, 0, 0, 0, nullptr, 4, s), MCMC_OK);
