@@ -755,7 +755,7 @@ static int check_grouped_dims(int64_t rows, int n_groups, int n_in, int n_out) {
 int64_t mcmc_grouped_linear_workspace_bytes(int dtype, int64_t rows, int n_groups, int n_in, int n_out) {
     if (int rc = check_operand_dtype(dtype)) return rc;
     if (int rc = check_grouped_dims(rows, n_groups, n_in, n_out)) return rc;
-    return grouped_linear_workspace_bytes(dtype, rows, n_groups, n_in, n_out);
+    return grouped_linear_workspace_bytes(rows, n_groups, n_in, n_out);
 }
 
 int mcmc_grouped_linear_forward(mcmc_ctx* ctx, int dtype, const void* x, int64_t ld_x, int64_t rows, const int32_t* order, const int32_t* offsets,
@@ -794,7 +794,7 @@ int mcmc_grouped_linear_grad_weight(mcmc_ctx* ctx, int dtype, const void* dy, in
     MCMC_REQUIRE(rows == 0 || (dy && x), "dy / x is NULL");
     MCMC_REQUIRE(aligned_for(dtype, dy) && aligned_for(dtype, x) && aligned_for(dtype, dweight) && aligned_for(dtype, dbias),
                  "dy, x, dweight and dbias must be aligned to their elements");
-    if (grouped_linear_workspace_bytes(dtype, rows, n_groups, n_in, n_out) > 0)
+    if (grouped_linear_workspace_bytes(rows, n_groups, n_in, n_out) > 0)
         MCMC_REQUIRE(workspace && aligned16(workspace), "workspace must be 16-byte aligned device memory (mcmc_grouped_linear_workspace_bytes)");
     return launch_grouped_linear_grad_weight(dtype, dy, ld_dy, x, ld_x, rows, order, offsets, n_groups, n_in, n_out, dweight, dbias, workspace,
                                              (hipStream_t)stream);

@@ -41,32 +41,36 @@ struct Args {
     int chunks;      // dW: partial sums there is room for
 };
 
-// ---- matrix instructions: 16 x 16 outputs, kc contraction elements per fragment --------------------------------------------
-// lane l holds row (l & 15) and kv consecutive elements from kv * (l >> 4); D: lane l holds column l & 15, rows 4 (l >> 4) + i
+// ---- matrix instructions: 16 x 16 outputs, 32 contraction elements ---------------------------------------------------------
+// a fragment: lane l holds row (l & 15) and eight consecutive elements from 8 (l >> 4); D: lane l holds column l & 15, rows
+// 4 (l >> 4) + i
 template <typename T>
 struct Frag;
 template <>
 struct Frag<__bf16> {
+    typedef __bf16 E;  // what the tiles in LDS hold
     typedef bf16x8 V;
-    static constexpr int kv = 8;
+    static constexpr int kPlanes = 1;
     static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 d) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, d, 0, 0, 0); }
 };
 template <>
 struct Frag<_Float16> {
+    typedef _Float16 E;
     typedef f16x8 V;
-    static constexpr int kv = 8;
+    static constexpr int kPlanes = 1;
     static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 d) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, d, 0, 0, 0); }
 };
+// fp32 on the bf16 pipe: the fp32 matrix instructions run at 1/16 of its rate.  x = h + m + l with h = x rounded to bf16's 8 bits, m =
+// the rest rounded likewise, l = what is left (at most 8 bits: exact, down to 2^-126); of the nine products the six down to h l +
+// m m + l h are summed in fp32, the small ones first, so that a short sum is rounded once.  Left out: m l + l m + l l, below
+// 2^-26 |x y|, a quarter of an fp32 rounding.  What rounds to an infinity has no such split (inf - inf): a workgroup that meets one
+// does its tile over, element by element.
 template <>
 struct Frag<float> {
-    typedef f32x4 V;
-    static constexpr int kv = 4;
-    // four 16x16x4 steps; step i takes element i of every lane: the same contraction index on both sides, in another order
-    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 d) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], d, 0, 0, 0);
-        return d;
-    }
+    typedef __bf16 E;
+    typedef bf16x8 V;
+    static constexpr int kPlanes = 3;
+    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 d) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, d, 0, 0, 0); }
 };
 
 // ---- tiles -----------------------------------------------------------------------------------------------------------------
@@ -127,137 +131,28 @@ __device__ __forceinline__ int row_at(const Args& a, int pos) {
 }
 
 constexpr int kThreads = 256;
-constexpr int BP = 64, BQ = 64;
 
-// 64 x 64 outputs per workgroup, 32 x 32 per wave; operands go through LDS with the contraction index contiguous
-template <typename T, int PRODUCT>
-__global__ __launch_bounds__(kThreads) void grouped_product_kernel(Args a) {
-    typedef Frag<T> F;
-    constexpr int BC = sizeof(T) == 2 ? 64 : 32, S = BC + 16 / (int)sizeof(T);
-    __shared__ T lp[BP * S], lq[BQ * S];
-    __shared__ int rows_p[BP], rows_c[BC];
-    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-    const int n_q = PRODUCT == kForward ? a.n_out : a.n_in, q_tiles = (n_q + BQ - 1) / BQ;
-    const int q0 = (int)(blockIdx.x % q_tiles) * BQ;
-    int run = blockIdx.x / q_tiles;  // row tile; dW: the group or chunk
-    int p0 = 0;                      // first output row of the tile
-    Tile tl;
-    if (PRODUCT == kGradWeight) {
-        const int p_tiles = (a.n_out + BP - 1) / BP;
-        p0 = run % p_tiles * BP;
-        run /= p_tiles;
-        if (a.chunk_rows) {
-            tl = find_tile(a.offsets, a.G, (int)a.rows, run, a.chunk_rows);
-            if (tl.g < 0 || tl.g >= a.G) return;
-        } else {
-            const int b = clamp_pos(a.offsets[run], 0, (int)a.rows);
-            tl = Tile{run, b, clamp_pos(a.offsets[run + 1], b, (int)a.rows)};
-        }
-    } else {
-        tl = find_tile(a.offsets, a.G, (int)a.rows, run, BP);
-        if (tl.g < 0) return;
-        if (t < BP) rows_p[t] = tl.first + t < tl.last ? row_at(a, tl.first + t) : -1;
-    }
-    const int n_p = PRODUCT == kGradWeight ? a.n_out : BP;
-    const int n_c = PRODUCT == kForward ? a.n_in : PRODUCT == kGradInput ? a.n_out : tl.last - tl.first;
-    const bool none = PRODUCT != kGradWeight && tl.g == a.G;
-    const T* P = static_cast<const T*>(a.p);
-    const T* Q = static_cast<const T*>(a.q);
-    if (PRODUCT != kGradWeight && !none) Q += (int64_t)tl.g * a.n_in * a.n_out;
-    f32x4 acc[2][2] = {}, accb[2] = {};
-    const int pw = 32 * (wv & 1), qw = 32 * (wv >> 1), fr = lane & 15, fk = F::kv * (lane >> 4);
-    typename F::V ones;
-#pragma unroll
-    for (int i = 0; i < F::kv; ++i) ones[i] = (T)1.0f;
-    __syncthreads();
-    for (int c0 = 0; c0 < (none ? 0 : n_c); c0 += BC) {
-        if (PRODUCT == kGradWeight) {
-            if (t < BC) rows_c[t] = c0 + t < n_c ? row_at(a, tl.first + c0 + t) : -1;
-            __syncthreads();
-            for (int i = t; i < BP * BC; i += kThreads) {
-                const int p = i % BP, c = i / BP, r = rows_c[c];
-                lp[p * S + c] = r >= 0 && p0 + p < n_p ? P[(int64_t)r * a.ld_p + p0 + p] : (T)0.0f;
-                lq[p * S + c] = r >= 0 && q0 + p < n_q ? Q[(int64_t)r * a.ld_q + q0 + p] : (T)0.0f;
-            }
-        } else {
-            for (int i = t; i < BP * BC; i += kThreads) {
-                const int c = i % BC, p = i / BC, r = rows_p[p];
-                lp[p * S + c] = r >= 0 && c0 + c < n_c ? P[(int64_t)r * a.ld_p + c0 + c] : (T)0.0f;
-            }
-            for (int i = t; i < BQ * BC; i += kThreads) {
-                if (PRODUCT == kForward) {
-                    const int c = i % BC, q = i / BC;
-                    lq[q * S + c] = q0 + q < n_q && c0 + c < n_c ? Q[(int64_t)(q0 + q) * a.ld_q + c0 + c] : (T)0.0f;
-                } else {
-                    const int q = i % BQ, c = i / BQ;
-                    lq[q * S + c] = q0 + q < n_q && c0 + c < n_c ? Q[(int64_t)(c0 + c) * a.ld_q + q0 + q] : (T)0.0f;
-                }
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < BC; k += 4 * F::kv) {
-            typename F::V fp[2], fq[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fp[i] = *reinterpret_cast<const typename F::V*>(lp + (pw + 16 * i + fr) * S + k + fk);
-                fq[i] = *reinterpret_cast<const typename F::V*>(lq + (qw + 16 * i + fr) * S + k + fk);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = F::mfma(fq[j], fp[i], acc[i][j]);
-            if (PRODUCT == kGradWeight && a.dbias && q0 == 0)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) accb[i] = F::mfma(ones, fp[i], accb[i]);
-        }
-        __syncthreads();
-    }
-    // lane: output row p = fr of fragment i, four consecutive q
-    const T* bias = PRODUCT == kForward && a.bias && !none ? static_cast<const T*>(a.bias) + (int64_t)tl.g * a.n_out : nullptr;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int p = pw + 16 * i + fr;
-        int64_t at;
-        if (PRODUCT == kGradWeight) {
-            if (p0 + p >= n_p) continue;
-            at = ((int64_t)run * a.n_out + p0 + p) * a.n_in;
-        } else {
-            if (rows_p[p] < 0) continue;
-            at = (int64_t)rows_p[p] * n_q;
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int q = q0 + qw + 16 * j + 4 * (lane >> 4) + e;
-                if (q >= n_q) continue;
-                float v = acc[i][j][e];
-                if (bias) v += (float)bias[q];
-                if (PRODUCT == kGradWeight && a.chunk_rows) a.part[at + q] = v;
-                else static_cast<T*>(a.out)[at + q] = (T)v;
-            }
-        if (PRODUCT == kGradWeight && a.dbias && q0 == 0 && qw == 0 && lane < 16) {
-            if (a.chunk_rows) a.part[(int64_t)a.chunks * a.n_out * a.n_in + (int64_t)run * a.n_out + p0 + p] = accb[i][0];
-            else static_cast<T*>(a.dbias)[(int64_t)tl.g * a.n_out + p0 + p] = (T)accb[i][0];
-        }
-    }
-}
-
-// ---- 16-bit types: large tiles, operands by LDS-DMA ------------------------------------------------------------------------
-// BP x BQ outputs per workgroup of WP x WQ waves, 64 contraction elements a step, two LDS stages: the loads of step t+1 run while
-// step t is multiplied, one barrier a step.  The tiles lie in LDS as they lie in memory, in 16-byte pieces:
-//   "rows"    [BP or BQ][64 c]   operands whose contraction index is contiguous (x, dy; W in the forward pass); fragments by
-//             ds_read_b128.  Piece s of row r holds chunk s ^ (r & 7): the eight lanes of a pass, eight rows, hit all banks.
-//   "columns" [64 c][BP or BQ]   operands whose output index is contiguous (W in dx; both in dW); fragments by ds_read_b64_tr_b16,
+// ---- the tile product ------------------------------------------------------------------------------------------------------
+// BP x BQ outputs per workgroup of WP x WQ waves, BC contraction elements a step.  The tiles lie in LDS as they lie in memory, in
+// 16-byte pieces of eight 16-bit elements (fp32: three planes of bf16):
+//   "rows"    [BP or BQ][BC]     operands whose contraction index is contiguous (x, dy; W in the forward pass); fragments by
+//             ds_read_b128.  The pieces of row r are permuted by turn(r): the rows a pass touches hit all banks.
+//   "columns" [BC][BP or BQ]     operands whose output index is contiguous (W in dx; both in dW); fragments by ds_read_b64_tr_b16,
 //             which hands each lane a column of four rows.  The 32-byte chunks of row c are permuted by spread(c): the eight rows a
 //             pass touches ({0-3, 8-11} + 4n) hit all banks.
-// DMA: every row starts on 16 bytes and holds whole 8-element chunks: the pieces go global -> LDS directly (the permutation is
-// on the global side, a wave-instruction fills 1 KiB of LDS in order), 16 zero bytes stand in for what lies past the contraction's
-// end.  Otherwise they pass through registers, element by element where a chunk crosses the end of a row.
+// 16-bit types, two LDS stages: the loads of step t+1 run while step t is multiplied, one barrier a step.
+//   DMA: every row starts on 16 bytes and holds whole 8-element chunks: the pieces go global -> LDS directly (the permutation is
+//   on the global side, a wave-instruction fills 1 KiB of LDS in order), 16 zero bytes stand in for what lies past the
+//   contraction's end.  Otherwise they pass through registers, element by element where a chunk crosses the end of a row.
+// fp32, one LDS stage (three planes are 48 KB at 128 x 128 x 32: two workgroups a CU, one multiplies while the other stages): the
+// loads of step t+1 are in registers while step t is multiplied, and are split on their way into LDS.
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 constexpr int kSegment = 1024;  // dW: row numbers in LDS, two segments, the next one loaded while one is used
 
+template <int BC>
+__device__ __forceinline__ int turn(int r) {  // permutation of the 16-byte pieces of row r
+    return BC == 64 ? r & 7 : (r >> 2) & 3;
+}
 template <int B>
 __device__ __forceinline__ int spread(int c) {  // bytes to xor: bits 5.. of the offset in row c
     if (B >= 128) return ((c & 3) | ((c >> 1) & 4)) << 5;
@@ -265,15 +160,40 @@ __device__ __forceinline__ int spread(int c) {  // bytes to xor: bits 5.. of the
     return 0;
 }
 
-__device__ __forceinline__ uint4 load_piece(const void* p, int n) {  // n of its eight 2-byte elements exist
-    union { uint4 v; uint16_t h[8]; } u;
+// eight elements in registers; n of them exist
+template <typename T>
+struct Piece {
+    T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T* p, int n) {
+    Piece<T> u;
     if (n >= 8) {
-        __builtin_memcpy(&u.v, p, 16);
+        __builtin_memcpy(u.v, p, sizeof(u.v));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u.h[i] = i < n ? static_cast<const uint16_t*>(p)[i] : (uint16_t)0;
+        for (int i = 0; i < 8; ++i) u.v[i] = i < n ? p[i] : (T)0.0f;
     }
-    return u.v;
+    return u;
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(char* at, int plane_bytes, const Piece<T>& u, bool& infinite) {
+    if constexpr (sizeof(T) == 2) {
+        __builtin_memcpy(__builtin_assume_aligned(at, 16), u.v, 16);
+    } else {
+        bf16x8 h, m, l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            h[i] = (__bf16)u.v[i];
+            const float hi = (float)h[i], rest = u.v[i] - hi;
+            infinite |= __builtin_isinf(hi);
+            m[i] = (__bf16)rest;
+            l[i] = (__bf16)(rest - (float)m[i]);
+        }
+        *reinterpret_cast<bf16x8*>(at) = h;
+        *reinterpret_cast<bf16x8*>(at + plane_bytes) = m;
+        *reinterpret_cast<bf16x8*>(at + 2 * plane_bytes) = l;
+    }
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -296,14 +216,16 @@ __device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t n) {
 template <typename T, int PRODUCT, int BP, int BQ, int WP, int WQ, bool DMA>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     typedef Frag<T> F;
-    constexpr int BC = 64, NW = WP * WQ, NT = 64 * NW;
+    typedef typename F::V V;
+    constexpr bool kWide = sizeof(T) == 4;
+    constexpr int BC = kWide ? 32 : 64, NW = WP * WQ, NT = 64 * NW, kStages = kWide ? 1 : 2;
     constexpr bool kPCols = PRODUCT == kGradWeight, kQCols = PRODUCT != kForward;
-    constexpr int kPBytes = BP * BC * 2, kQBytes = BQ * BC * 2, kStage = kPBytes + kQBytes;
+    constexpr int kPBytes = BP * BC * 2, kQBytes = BQ * BC * 2, kStage = (kPBytes + kQBytes) * F::kPlanes;
     constexpr int NP = kPBytes / 1024 / NW, NQ = kQBytes / 1024 / NW;  // 1-KiB pieces of a stage each wave loads
     constexpr int FP = BP / WP / 16, FQ = BQ / WQ / 16;
-    static_assert(NP >= 1 && NQ >= 1 && FP >= 1 && FQ >= 1, "every wave loads and multiplies");
+    static_assert(NP >= 1 && NQ >= 1 && FP >= 1 && FQ >= 1 && !(DMA && kWide), "every wave loads and multiplies; fp32 is split in registers");
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int* const rows_lds = reinterpret_cast<int*>(smem + 2 * kStage);  // dW: [2][kSegment] row numbers; else [BP]
+    int* const rows_lds = reinterpret_cast<int*>(smem + kStages * kStage);  // dW: [2][kSegment] row numbers; else [BP]
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int rows = (int)a.rows;
     const int n_q = PRODUCT == kForward ? a.n_out : a.n_in, n_p = PRODUCT == kGradWeight ? a.n_out : BP;
@@ -352,36 +274,33 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     const T* const Q = static_cast<const T*>(a.q) + (PRODUCT != kGradWeight && !none ? (int64_t)tl.g * a.n_in * a.n_out : 0);
     const T* const zeros = reinterpret_cast<const T*>(&kZeros);
 
-    // ---- where this lane's pieces come from: an address at step 0, and the first contraction index it needs
-    const T *src_p[NP], *src_q[NQ];
-    int c_p[NP], c_q[NQ];  // "columns": row of the tile; "rows": first element of the chunk
-    int w_p[NP], w_q[NQ];  // !DMA, "columns": elements of the chunk that exist
+    // ---- where this lane's pieces come from.  "rows": the chunk's address at step 0 and its first element; "columns": its row of the
+    // tile and its first column (columns past the end: any, their products are not stored)
+    const T *src_p[kPCols ? 1 : NP], *src_q[kQCols ? 1 : NQ];
+    int c_p[NP], c_q[NQ], col_p[NP], col_q[NQ];
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
         const int piece = (wave * NP + n) * 64 + lane;
-        if (kPCols) {
+        if constexpr (kPCols) {
             c_p[n] = piece / (BP / 8);
-            const int col = p0 + 8 * ((piece % (BP / 8)) ^ (spread<BP>(c_p[n]) >> 4));
-            w_p[n] = n_p - col;
-            src_p[n] = P + (DMA ? (col + 8 <= n_p ? col : 0) : (w_p[n] > 0 ? col : 0));  // columns past the end: any, not stored
+            col_p[n] = p0 + 8 * ((piece % (BP / 8)) ^ (spread<BP>(c_p[n]) >> 4));
+            if (DMA && col_p[n] >= n_p) col_p[n] = 0;
         } else {
-            const int r = piece >> 3, row = rows_lds[r] < 0 ? 0 : rows_lds[r];  // rows past the end: any, not stored
-            c_p[n] = 8 * ((piece & 7) ^ (r & 7));
+            const int r = piece / (BC / 8), row = rows_lds[r] < 0 ? 0 : rows_lds[r];  // rows past the end: any, not stored
+            c_p[n] = 8 * ((piece % (BC / 8)) ^ turn<BC>(r));
             src_p[n] = P + (int64_t)row * a.ld_p + c_p[n];
         }
     }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int piece = (wave * NQ + n) * 64 + lane;
-        if (kQCols) {
+        if constexpr (kQCols) {
             c_q[n] = piece / (BQ / 8);
-            const int col = q0 + 8 * ((piece % (BQ / 8)) ^ (spread<BQ>(c_q[n]) >> 4));
-            w_q[n] = n_q - col;
-            src_q[n] = Q + (DMA ? (col + 8 <= n_q ? col : 0) : (w_q[n] > 0 ? col : 0));
-            if (PRODUCT == kGradInput) src_q[n] += (int64_t)c_q[n] * a.ld_q;
+            col_q[n] = q0 + 8 * ((piece % (BQ / 8)) ^ (spread<BQ>(c_q[n]) >> 4));
+            if (DMA && col_q[n] >= n_q) col_q[n] = 0;
         } else {
-            const int r = piece >> 3, row = q0 + r < n_q ? q0 + r : n_q - 1;
-            c_q[n] = 8 * ((piece & 7) ^ (r & 7));
+            const int r = piece / (BC / 8), row = q0 + r < n_q ? q0 + r : n_q - 1;
+            c_q[n] = 8 * ((piece % (BC / 8)) ^ turn<BC>(r));
             src_q[n] = Q + (int64_t)row * a.ld_q + c_q[n];
         }
     }
@@ -400,18 +319,19 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         const int r = a.order ? rows_lds[c & (2 * kSegment - 1)] : tl.first + c;
         return (unsigned)r < (unsigned)rows ? r : -1;
     };
-    uint4 hold_p[DMA ? 1 : NP], hold_q[DMA ? 1 : NQ];
+    Piece<T> hold_p[DMA ? 1 : NP], hold_q[DMA ? 1 : NQ];
+    bool infinite = false;
     auto load = [&](int step, int stage) {  // DMA: into LDS; otherwise into hold_*
         const int c0 = step * BC;
-        const unsigned to_p = lds_address(smem + stage * kStage) + wave * NP * 1024, to_q = lds_address(smem + stage * kStage + kPBytes) + wave * NQ * 1024;
+        const unsigned to_p = lds_address(smem + stage * kStage) + wave * NP * 1024, to_q = to_p + kPBytes + wave * (NQ - NP) * 1024;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const T* p;
-            int have;  // elements of the chunk inside the contraction
-            if (kPCols) {
+            int have;  // elements of the chunk that exist (DMA: all or none)
+            if constexpr (kPCols) {
                 const int r = row_of(c0 + c_p[n]);
-                have = r >= 0 ? (DMA ? 8 : w_p[n]) : 0;
-                p = src_p[n] + (int64_t)r * a.ld_p;
+                have = r >= 0 ? (DMA ? 8 : n_p - col_p[n]) : 0;
+                p = P + (int64_t)r * a.ld_p + col_p[n];
             } else {
                 have = n_c - c0 - c_p[n];
                 p = src_p[n] + c0;
@@ -423,13 +343,10 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         for (int n = 0; n < NQ; ++n) {
             const T* q;
             int have;
-            if (PRODUCT == kGradWeight) {
-                const int r = row_of(c0 + c_q[n]);
-                have = r >= 0 ? (DMA ? 8 : w_q[n]) : 0;
-                q = src_q[n] + (int64_t)r * a.ld_q;
-            } else if (PRODUCT == kGradInput) {
-                have = c0 + c_q[n] < n_c ? (DMA ? 8 : w_q[n]) : 0;
-                q = src_q[n] + (int64_t)c0 * a.ld_q;
+            if constexpr (kQCols) {
+                const int c = c0 + c_q[n], r = PRODUCT == kGradWeight ? row_of(c) : c < n_c ? c : -1;
+                have = r >= 0 ? (DMA ? 8 : n_q - col_q[n]) : 0;
+                q = Q + (int64_t)r * a.ld_q + col_q[n];
             } else {
                 have = n_c - c0 - c_q[n];
                 q = src_q[n] + c0;
@@ -441,29 +358,60 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     auto store = [&](int stage) {
         char* s = smem + stage * kStage;
 #pragma unroll
-        for (int n = 0; n < NP; ++n) *reinterpret_cast<uint4*>(s + ((wave * NP + n) * 64 + lane) * 16) = hold_p[DMA ? 0 : n];
+        for (int n = 0; n < NP; ++n) store_piece(s + ((wave * NP + n) * 64 + lane) * 16, kPBytes, hold_p[DMA ? 0 : n], infinite);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) *reinterpret_cast<uint4*>(s + kPBytes + ((wave * NQ + n) * 64 + lane) * 16) = hold_q[DMA ? 0 : n];
+        for (int n = 0; n < NQ; ++n) store_piece(s + F::kPlanes * kPBytes + ((wave * NQ + n) * 64 + lane) * 16, kQBytes, hold_q[DMA ? 0 : n], infinite);
     };
 
     // ---- fragments
     const int pw = BP / WP * (wave % WP), qw = BQ / WQ * (wave / WP), fr = lane & 15, kg = lane >> 4;
-    auto frag = [&](auto cols, auto width, const char* tile, int first, int i, int kk) -> typename F::V {
+    auto frag = [&](auto cols, auto width, const char* tile, int first, int i, int kk) -> V {
         constexpr bool C = decltype(cols)::value;
         constexpr int B = decltype(width)::value;
         if constexpr (C) {
             const int c = 32 * kk + 8 * kg + (fr >> 2);  // rows c and c + 4
-            return columns_frag<typename F::V>(tile + c * (2 * B) + ((2 * (first + 16 * i)) ^ spread<B>(8 * kg + (fr >> 2))) + 8 * (fr & 3), 4 * 2 * B);
+            return columns_frag<V>(tile + c * (2 * B) + ((2 * (first + 16 * i)) ^ spread<B>(8 * kg + (fr >> 2))) + 8 * (fr & 3), 4 * 2 * B);
         } else {
             const int r = first + 16 * i + fr;
-            return *reinterpret_cast<const typename F::V*>(tile + r * (2 * BC) + (((4 * kk + kg) ^ (fr & 7)) << 4));
+            return *reinterpret_cast<const V*>(tile + r * (2 * BC) + (((4 * kk + kg) ^ turn<BC>(fr)) << 4));
         }
     };
     f32x4 acc[FP][FQ] = {}, accb[FP] = {};
+    // db: the sum of dy's columns as one more product, by ones; a long plain sum loses more than a product's, so every kSegment rows
+    // the running sum goes into a second one (rounding of n terms ~ sqrt(n / 1024) + sqrt(256) instead of sqrt(n / 4) steps)
+    float sumb[FP] = {};
     const bool sum_bias = PRODUCT == kGradWeight && a.dbias && q0 == 0 && qw == 0;
-    typename F::V ones;
+    V ones;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ones[i] = (T)1.0f;
+    for (int i = 0; i < 8; ++i) ones[i] = (typename F::E)1.0f;
+    auto multiply = [&](const char* tp) {
+        const char* tq = tp + F::kPlanes * kPBytes;
+#pragma unroll
+        for (int kk = 0; kk < BC / 32; ++kk) {
+            V fq[F::kPlanes][FQ];
+#pragma unroll
+            for (int l = 0; l < F::kPlanes; ++l)
+#pragma unroll
+                for (int j = 0; j < FQ; ++j)
+                    fq[l][j] = frag(std::integral_constant<bool, kQCols>(), std::integral_constant<int, BQ>(), tq + l * kQBytes, qw, j, kk);
+#pragma unroll
+            for (int l = F::kPlanes - 1; l >= 0; --l) {
+                V fp[FP];
+#pragma unroll
+                for (int i = 0; i < FP; ++i)
+                    fp[i] = frag(std::integral_constant<bool, kPCols>(), std::integral_constant<int, BP>(), tp + l * kPBytes, pw, i, kk);
+#pragma unroll
+                for (int m = F::kPlanes - 1 - l; m >= 0; --m)
+#pragma unroll
+                    for (int i = 0; i < FP; ++i)
+#pragma unroll
+                        for (int j = 0; j < FQ; ++j) acc[i][j] = F::mfma(fq[m][j], fp[i], acc[i][j]);
+                if (sum_bias)
+#pragma unroll
+                    for (int i = 0; i < FP; ++i) accb[i] = F::mfma(ones, fp[i], accb[i]);
+            }
+        }
+    };
 
     if (steps > 0) {
         fetch_segment(0);
@@ -472,38 +420,66 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             __syncthreads();
         }
         load(0, 0);
-        if (!DMA) store(0);
+        if (!DMA && !kWide) store(0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         barrier_lds_only();
     }
     for (int s = 0; s < steps; ++s) {
-        if (s % (kSegment / BC) == 0) fetch_segment(s / (kSegment / BC) + 1);  // the segment before s's is no longer read
-        if (s + 1 < steps) load(s + 1, (s + 1) & 1);
-        const char* tp = smem + (s & 1) * kStage;
-        const char* tq = tp + kPBytes;
-#pragma unroll
-        for (int kk = 0; kk < BC / 32; ++kk) {
-            typename F::V fp[FP], fq[FQ];
-#pragma unroll
-            for (int j = 0; j < FQ; ++j) fq[j] = frag(std::integral_constant<bool, kQCols>(), std::integral_constant<int, BQ>(), tq, qw, j, kk);
-#pragma unroll
-            for (int i = 0; i < FP; ++i) fp[i] = frag(std::integral_constant<bool, kPCols>(), std::integral_constant<int, BP>(), tp, pw, i, kk);
-#pragma unroll
-            for (int i = 0; i < FP; ++i)
-#pragma unroll
-                for (int j = 0; j < FQ; ++j) acc[i][j] = F::mfma(fq[j], fp[i], acc[i][j]);
+        if (s % (kSegment / BC) == 0) {
+            fetch_segment(s / (kSegment / BC) + 1);  // the segment before s's is no longer read
             if (sum_bias)
 #pragma unroll
-                for (int i = 0; i < FP; ++i) accb[i] = F::mfma(ones, fp[i], accb[i]);
+                for (int i = 0; i < FP; ++i) sumb[i] += accb[i][0], accb[i] = f32x4{};
         }
-        if (!DMA && s + 1 < steps) store((s + 1) & 1);
+        if (kWide) {
+            store(0);
+            barrier_lds_only();
+        }
+        if (s + 1 < steps) load(s + 1, (s + 1) & 1);
+        multiply(smem + (kWide ? 0 : s & 1) * kStage);
+        if (!DMA && !kWide && s + 1 < steps) store((s + 1) & 1);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         barrier_lds_only();
+    }
+    if constexpr (kWide) {
+        // an infinity among the operands: the sums again, element by element from memory (rare, and as slow as that sounds)
+        if (__syncthreads_or(infinite)) {
+            for (int i = 0; i < FP; ++i) {
+                const int p = pw + 16 * i + fr, row = kPCols ? 0 : rows_lds[p];
+                sumb[i] = 0.0f;
+                accb[i] = f32x4{};
+                for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{};
+                if (kPCols ? p0 + p >= n_p : row < 0) continue;
+                for (int c = 0; c < n_c; ++c) {
+                    const int r = kPCols ? (a.order ? a.order[tl.first + c] : tl.first + c) : row;
+                    if ((unsigned)r >= (unsigned)rows) continue;
+                    const float x = P[(int64_t)r * a.ld_p + (kPCols ? p0 + p : c)];
+                    sumb[i] += x;
+                    for (int j = 0; j < FQ; ++j)
+                        for (int e = 0; e < 4; ++e) {
+                            const int q = q0 + qw + 16 * j + 4 * kg + e;
+                            if (q >= n_q) continue;
+                            const int64_t at = PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)(PRODUCT == kGradInput ? c : r) * a.ld_q + q;
+                            acc[i][j][e] = fmaf(x, Q[at], acc[i][j][e]);
+                        }
+                }
+            }
+        }
     }
 
     // ---- lane: output row fr of fragment i, four consecutive q
     const T* bias = PRODUCT == kForward && a.bias && !none ? static_cast<const T*>(a.bias) + (int64_t)tl.g * a.n_out : nullptr;
     const bool whole = n_q % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;  // four results are one 8-byte store
+    if (bias)
+#pragma unroll
+        for (int j = 0; j < FQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int q = q0 + qw + 16 * j + 4 * kg + e;
+                const float b = (float)bias[q < n_q ? q : 0];
+#pragma unroll
+                for (int i = 0; i < FP; ++i) acc[i][j][e] += b;
+            }
 #pragma unroll
     for (int i = 0; i < FP; ++i) {
         const int p = pw + 16 * i + fr;
@@ -518,10 +494,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < FQ; ++j) {
             const int q = q0 + qw + 16 * j + 4 * kg;
-            f32x4 v = acc[i][j];
-            if (bias)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] += q + e < n_q ? (float)bias[q + e] : 0.0f;
+            const f32x4 v = acc[i][j];
             if (PRODUCT == kGradWeight && a.chunk_rows) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -536,13 +509,15 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             }
         }
         if (sum_bias && lane < 16) {
-            if (a.chunk_rows) a.part[(int64_t)a.chunks * a.n_out * a.n_in + (int64_t)run * a.n_out + p0 + p] = accb[i][0];
-            else static_cast<T*>(a.dbias)[(int64_t)tl.g * a.n_out + p0 + p] = (T)accb[i][0];
+            const float v = sumb[i] + accb[i][0];
+            if (a.chunk_rows) a.part[(int64_t)a.chunks * a.n_out * a.n_in + (int64_t)run * a.n_out + p0 + p] = v;
+            else static_cast<T*>(a.dbias)[(int64_t)tl.g * a.n_out + p0 + p] = (T)v;
         }
     }
 }
 
-// dW[g] = the sum of group g's chunks in their order; the same for db.  One workgroup: 256 elements of one group.
+// dW[g] = the sum of group g's chunks in their order, in 64 bits (free: the kernel waits for memory); the same for db.  One
+// workgroup: 256 elements of one group.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void grouped_sum_kernel(Args a) {
     const int64_t n = (int64_t)a.n_out * a.n_in, all = n + (a.dbias ? a.n_out : 0);
@@ -554,29 +529,26 @@ __global__ __launch_bounds__(kThreads) void grouped_sum_kernel(Args a) {
     if (i >= all) return;
     const float* src = i < n ? a.part + i : a.part + (int64_t)a.chunks * n + (i - n);
     const int64_t step = i < n ? n : a.n_out;
-    float s = 0.0f;
-    for (int c = first; c < last; ++c) s += src[c * step];
+    double s = 0.0;
+    for (int c = first; c < last; ++c) s += (double)src[c * step];
     if (i < n) static_cast<T*>(a.out)[g * n + i] = (T)s;
     else static_cast<T*>(a.dbias)[(int64_t)g * a.n_out + (i - n)] = (T)s;
 }
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// The products of 16-bit types run on 128 x 128 or 256 x 256 tiles, fp32 on 64 x 64.
 struct Shape {
     int bp, bq;
 };
-Shape shape_of(int dtype, int product, bool dma, int64_t rows, int G, int n_in, int n_out) {
-    if (dtype == MCMC_DT_F32) return Shape{BP, BQ};
+Shape shape_of(int product, bool dma, int64_t rows, int G, int n_in, int n_out) {
     const int64_t n_p = product == kGradWeight ? n_out : rows / G, n_q = product == kForward ? n_out : n_in;
     const int64_t tiles = (product == kGradWeight ? (int64_t)ceil_div(n_out, 256) * G : rows / 256) * ceil_div(n_q, 256);
     return dma && n_p >= 192 && n_q >= 192 && tiles >= 256 ? Shape{256, 256} : Shape{128, 128};
 }
 
 // rows per partial sum of dW: 0 (no split) when the output tiles alone fill the chip
-int chunk_rows_of(int dtype, int64_t rows, int G, int n_in, int n_out) {
-    const Shape sh = shape_of(dtype, kGradWeight, false, rows, G, n_in, n_out);
-    const int64_t tiles = (int64_t)ceil_div(n_out, sh.bp) * ceil_div(n_in, sh.bq);
+int chunk_rows_of(int64_t rows, int G, int n_in, int n_out) {
+    const int64_t tiles = (int64_t)ceil_div(n_out, 128) * ceil_div(n_in, 128);
     if (tiles * G >= 512 || rows <= 512) return 0;
     int64_t per = ceil_div(rows * tiles, 1024);
     per = (per + 255) / 256 * 256;
@@ -589,10 +561,10 @@ int check_grid(int64_t blocks) {
     return MCMC_OK;
 }
 
-template <typename T, int PRODUCT, int TP, int TQ, int WP, int WQ, bool DMA>
+template <typename T, int PRODUCT, int BP, int BQ, int WP, int WQ, bool DMA>
 int launch_tile(unsigned blocks, const Args& a, hipStream_t s) {
-    const size_t lds = 2 * (size_t)(TP + TQ) * 128 + (PRODUCT == kGradWeight ? 2 * kSegment : TP) * sizeof(int);
-    const auto kern = grouped_tile_kernel<T, PRODUCT, TP, TQ, WP, WQ, DMA>;
+    const size_t lds = (sizeof(T) == 4 ? 3 * 64 : 2 * 128) * (size_t)(BP + BQ) + (PRODUCT == kGradWeight ? 2 * kSegment : BP) * sizeof(int);
+    const auto kern = grouped_tile_kernel<T, PRODUCT, BP, BQ, WP, WQ, DMA>;
     if (int rc = ensure_dyn_lds((const void*)kern, lds, "grouped_tile_kernel")) return rc;
     kern<<<blocks, 64 * WP * WQ, lds, s>>>(a);
     return check_launch("grouped_tile_kernel");
@@ -606,20 +578,18 @@ bool whole_chunks(int product, const Args& a) {
 
 template <typename T, int PRODUCT>
 int launch_product(const Args& a, Shape sh, bool dma, unsigned blocks, hipStream_t s) {
-    if constexpr (sizeof(T) == 4) {
-        grouped_product_kernel<T, PRODUCT><<<blocks, kThreads, 0, s>>>(a);
-        return check_launch("grouped_product_kernel");
-    } else {
+    if constexpr (sizeof(T) == 2) {
         if (sh.bp == 256) return launch_tile<T, PRODUCT, 256, 256, 2, 4, true>(blocks, a, s);
-        return dma ? launch_tile<T, PRODUCT, 128, 128, 2, 2, true>(blocks, a, s) : launch_tile<T, PRODUCT, 128, 128, 2, 2, false>(blocks, a, s);
+        if (dma) return launch_tile<T, PRODUCT, 128, 128, 2, 2, true>(blocks, a, s);
     }
+    return launch_tile<T, PRODUCT, 128, 128, 2, 2, false>(blocks, a, s);
 }
 
 template <typename T>
-int launch(int dtype, int product, const Args& a, hipStream_t s) {
+int launch(int product, const Args& a, hipStream_t s) {
     const int n_q = product == kForward ? a.n_out : a.n_in;
     const bool dma = sizeof(T) == 2 && whole_chunks(product, a);
-    const Shape sh = shape_of(dtype, product, dma, a.rows, a.G, a.n_in, a.n_out);
+    const Shape sh = shape_of(product, dma, a.rows, a.G, a.n_in, a.n_out);
     const int64_t runs = product == kGradWeight ? (int64_t)ceil_div(a.n_out, sh.bp) * (a.chunk_rows ? a.chunks : a.G)
                                                 : a.rows / sh.bp + (a.G + 1 < a.rows ? a.G + 1 : a.rows);
     const int64_t blocks = runs * ceil_div(n_q, sh.bq);
@@ -635,9 +605,9 @@ int launch(int dtype, int product, const Args& a, hipStream_t s) {
 }
 
 int launch_typed(int dtype, int product, const Args& a, hipStream_t s) {
-    if (dtype == MCMC_DT_F32) return launch<float>(dtype, product, a, s);
-    if (dtype == MCMC_DT_BF16) return launch<__bf16>(dtype, product, a, s);
-    return launch<_Float16>(dtype, product, a, s);
+    if (dtype == MCMC_DT_F32) return launch<float>(product, a, s);
+    if (dtype == MCMC_DT_BF16) return launch<__bf16>(product, a, s);
+    return launch<_Float16>(product, a, s);
 }
 
 }  // namespace
@@ -652,14 +622,14 @@ int launch_grouped_linear_grad_input(int dtype, const void* dy, int64_t ld_dy, i
     return launch_typed(dtype, kGradInput, Args{dy, weight, nullptr, dx, nullptr, nullptr, order, offsets, ld_dy, n_in, rows, G, n_in, n_out, 0, 0}, s);
 }
 
-int64_t grouped_linear_workspace_bytes(int dtype, int64_t rows, int G, int n_in, int n_out) {
-    const int per = chunk_rows_of(dtype, rows, G, n_in, n_out);
+int64_t grouped_linear_workspace_bytes(int64_t rows, int G, int n_in, int n_out) {
+    const int per = chunk_rows_of(rows, G, n_in, n_out);
     return per ? (int64_t)chunks_of(rows, G, per) * ((int64_t)n_in + 1) * n_out * 4 : 0;
 }
 
 int launch_grouped_linear_grad_weight(int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows, const int* order,
                                       const int* offsets, int G, int n_in, int n_out, void* dweight, void* dbias, void* ws, hipStream_t s) {
-    const int per = chunk_rows_of(dtype, rows, G, n_in, n_out);
+    const int per = chunk_rows_of(rows, G, n_in, n_out);
     return launch_typed(dtype, kGradWeight,
                         Args{dy, x, nullptr, dweight, dbias, static_cast<float*>(ws), order, offsets, ld_dy, ld_x, rows, G, n_in, n_out, per,
                              per ? chunks_of(rows, G, per) : 0},

@@ -545,3 +545,30 @@ def test_offsets_beyond_32_bits(dtype):
     keep = keep_flags(9, 1, 5, K, 0.5, row_begin=R - 5)
     assert torch.equal(d[-5:], torch.where(keep, x[-5:] * 2, torch.zeros_like(x[-5:])))
     assert not d[:-5].any()
+
+
+@pytest.mark.parametrize("K, N", [(40, 33), (256, 128)])
+def test_fp32_infinities_and_the_whole_range(K, N):
+    """fp32 products follow fp32's rules for infinities (inf * 1 = inf, inf - inf and inf * 0 = NaN), in the rows and columns they reach
+    and nowhere else, and keep their accuracy at the ends of the exponent range."""
+    R, G = 300, 3
+    x, w, b, dy, groups, ids = linear_case(R, G, K, N, FP32, 500)
+    x, w, dy = x.clone(), w.clone(), dy.clone()
+    x[5, 3], x[9, 0] = float("inf"), -float("inf")
+    w[1, 2, 1] = float("inf")
+    dy[20, 4] = -float("inf")
+    got = run_linear(x, w, b, dy, groups)
+    ref, mag = linear_reference(x, w, b, dy, ids)
+    for n in ref:
+        fine = ref[n].isfinite()
+        assert not fine.all()
+        assert torch.equal(got[n].isnan(), ref[n].isnan()) and torch.equal(got[n].isinf(), ref[n].isinf()), n
+        assert torch.equal(got[n][ref[n].isinf()].sign().double(), ref[n][ref[n].isinf()].sign()), n
+        check(got[n][fine], ref[n][fine], mag[n][fine] * U, n)
+    for sx, sw in ((2.0 ** 120, 2.0 ** -100), (2.0 ** -90, 2.0 ** 60), (3.4e38 / 6, 2.0 ** -20)):
+        x2, w2 = torch.randn(R, K, generator=gen(1), device=DEV).clamp(-6, 6) * sx, w * 0 + sw * 0.5
+        w2[:, :, ::3] *= -0.37
+        got = run_linear(x2, w2, b * 0, dy.clamp(-3, 3), groups)
+        ref, mag = linear_reference(x2, w2, b * 0, dy.clamp(-3, 3), ids)
+        for n in ("y", "dx"):
+            check(got[n], ref[n], mag[n] * U, n)
