@@ -46,6 +46,24 @@ struct Args {
 // 4 (l >> 4) + i
 template <typename T>
 struct Frag;
+// s + the sum of a fragment's eight elements
+__device__ __forceinline__ float add_elements(bf16x8 v, float s) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+    s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[0], v[1]}, one, s, false);
+    s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[2], v[3]}, one, s, false);
+    s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[4], v[5]}, one, s, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[6], v[7]}, one, s, false);
+}
+__device__ __forceinline__ float add_elements(f16x8 v, float s) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+    s = __builtin_amdgcn_fdot2(f16x2{v[0], v[1]}, one, s, false);
+    s = __builtin_amdgcn_fdot2(f16x2{v[2], v[3]}, one, s, false);
+    s = __builtin_amdgcn_fdot2(f16x2{v[4], v[5]}, one, s, false);
+    return __builtin_amdgcn_fdot2(f16x2{v[6], v[7]}, one, s, false);
+}
+
 template <>
 struct Frag<__bf16> {
     typedef __bf16 E;  // what the tiles in LDS hold
@@ -151,7 +169,7 @@ constexpr int kSegment = 1024;  // dW: row numbers in LDS, two segments, the nex
 
 template <int BC>
 __device__ __forceinline__ int turn(int r) {  // permutation of the 16-byte pieces of row r
-    return BC == 64 ? r & 7 : (r >> 2) & 3;
+    return BC == 64 ? r & 7 : -(r >> 2) & 3;
 }
 template <int B>
 __device__ __forceinline__ int spread(int c) {  // bytes to xor: bits 5.. of the offset in row c
@@ -172,7 +190,10 @@ __device__ __forceinline__ Piece<T> load_piece(const T* p, int n) {
         __builtin_memcpy(u.v, p, sizeof(u.v));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u.v[i] = i < n ? p[i] : (T)0.0f;
+        for (int i = 0; i < 8; ++i) {  // (a read that always happens, of the first element or of zeros: no branch per element)
+            const T x = n > 0 ? p[i < n ? i : 0] : (T)0.0f;
+            u.v[i] = i < n ? x : (T)0.0f;
+        }
     }
     return u;
 }
@@ -207,25 +228,33 @@ __device__ __forceinline__ V columns_frag(const char* p, int four_rows) {
     return __builtin_bit_cast(V, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
 }
 
+// until at most N of this wave's loads (global -> LDS ones included) are in flight; they complete in the order of their issue
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // workgroup id -> tile id: ids go round the eight XCDs, each XCD gets a contiguous run of tiles (its L2 sees neighbours)
 __device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t n) {
     const int64_t x = id & 7, i = id >> 3, q = n >> 3, r = n & 7;
     return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
 }
 
-template <typename T, int PRODUCT, int BP, int BQ, int WP, int WQ, bool DMA>
+template <typename T, int PRODUCT, int BP, int BQ, int WP, int WQ, bool DMA, int BC, int STAGES>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     typedef Frag<T> F;
     typedef typename F::V V;
     constexpr bool kWide = sizeof(T) == 4;
-    constexpr int BC = kWide ? 32 : 64, NW = WP * WQ, NT = 64 * NW, kStages = kWide ? 1 : 2;
+    constexpr int NW = WP * WQ, NT = 64 * NW;
+    constexpr bool kAhead = STAGES == 1;  // one stage: the next step waits in registers
+    static_assert(DMA ? STAGES >= 2 : STAGES <= 2, "");
     constexpr bool kPCols = PRODUCT == kGradWeight, kQCols = PRODUCT != kForward;
     constexpr int kPBytes = BP * BC * 2, kQBytes = BQ * BC * 2, kStage = (kPBytes + kQBytes) * F::kPlanes;
     constexpr int NP = kPBytes / 1024 / NW, NQ = kQBytes / 1024 / NW;  // 1-KiB pieces of a stage each wave loads
     constexpr int FP = BP / WP / 16, FQ = BQ / WQ / 16;
     static_assert(NP >= 1 && NQ >= 1 && FP >= 1 && FQ >= 1 && !(DMA && kWide), "every wave loads and multiplies; fp32 is split in registers");
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int* const rows_lds = reinterpret_cast<int*>(smem + kStages * kStage);  // dW: [2][kSegment] row numbers; else [BP]
+    int* const rows_lds = reinterpret_cast<int*>(smem + STAGES * kStage);  // dW: [2][kSegment] row numbers; else [BP]
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int rows = (int)a.rows;
     const int n_q = PRODUCT == kForward ? a.n_out : a.n_in, n_p = PRODUCT == kGradWeight ? a.n_out : BP;
@@ -274,34 +303,27 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     const T* const Q = static_cast<const T*>(a.q) + (PRODUCT != kGradWeight && !none ? (int64_t)tl.g * a.n_in * a.n_out : 0);
     const T* const zeros = reinterpret_cast<const T*>(&kZeros);
 
-    // ---- where this lane's pieces come from.  "rows": the chunk's address at step 0 and its first element; "columns": its row of the
-    // tile and its first column (columns past the end: any, their products are not stored)
+    // ---- where this lane's pieces come from.  "rows": the chunk's address at step 0, kept.  "columns": row of the tile and first column,
+    // made from the lane number where they are used: kept in registers for all pieces they would crowd out the accumulators
+    // (`now_lane` is the lane number behind an empty asm statement, so that the compiler does not move the arithmetic out of the loop).
     const T *src_p[kPCols ? 1 : NP], *src_q[kQCols ? 1 : NQ];
-    int c_p[NP], c_q[NQ], col_p[NP], col_q[NQ];
+    int c_p = 0, c_q = 0;  // "rows": first element of the chunk at step 0 (every piece of a lane has the same one)
+    int now_lane = lane;
+    auto col_row = [&](int n, int np, int b) { return ((wave * np + n) * 64 + now_lane) / (b / 8); };
+    if constexpr (!kPCols) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-        const int piece = (wave * NP + n) * 64 + lane;
-        if constexpr (kPCols) {
-            c_p[n] = piece / (BP / 8);
-            col_p[n] = p0 + 8 * ((piece % (BP / 8)) ^ (spread<BP>(c_p[n]) >> 4));
-            if (DMA && col_p[n] >= n_p) col_p[n] = 0;
-        } else {
-            const int r = piece / (BC / 8), row = rows_lds[r] < 0 ? 0 : rows_lds[r];  // rows past the end: any, not stored
-            c_p[n] = 8 * ((piece % (BC / 8)) ^ turn<BC>(r));
-            src_p[n] = P + (int64_t)row * a.ld_p + c_p[n];
+        for (int n = 0; n < NP; ++n) {
+            const int piece = (wave * NP + n) * 64 + lane, r = piece / (BC / 8), row = rows_lds[r] < 0 ? 0 : rows_lds[r];
+            c_p = 8 * ((piece % (BC / 8)) ^ turn<BC>(r));
+            src_p[n] = P + (int64_t)row * a.ld_p + c_p;  // rows past the end: any, not stored
         }
     }
+    if constexpr (!kQCols) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const int piece = (wave * NQ + n) * 64 + lane;
-        if constexpr (kQCols) {
-            c_q[n] = piece / (BQ / 8);
-            col_q[n] = q0 + 8 * ((piece % (BQ / 8)) ^ (spread<BQ>(c_q[n]) >> 4));
-            if (DMA && col_q[n] >= n_q) col_q[n] = 0;
-        } else {
-            const int r = piece / (BC / 8), row = q0 + r < n_q ? q0 + r : n_q - 1;
-            c_q[n] = 8 * ((piece % (BC / 8)) ^ turn<BC>(r));
-            src_q[n] = Q + (int64_t)row * a.ld_q + c_q[n];
+        for (int n = 0; n < NQ; ++n) {
+            const int piece = (wave * NQ + n) * 64 + lane, r = piece / (BC / 8), row = q0 + r < n_q ? q0 + r : n_q - 1;
+            c_q = 8 * ((piece % (BC / 8)) ^ turn<BC>(r));
+            src_q[n] = Q + (int64_t)row * a.ld_q + c_q;
         }
     }
     // dW: row numbers of the run's positions 1024 s .. 1024 s + 1023 -> LDS
@@ -321,39 +343,60 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     };
     Piece<T> hold_p[DMA ? 1 : NP], hold_q[DMA ? 1 : NQ];
     bool infinite = false;
-    auto load = [&](int step, int stage) {  // DMA: into LDS; otherwise into hold_*
-        const int c0 = step * BC;
-        const unsigned to_p = lds_address(smem + stage * kStage) + wave * NP * 1024, to_q = to_p + kPBytes + wave * (NQ - NP) * 1024;
+    // dW: the rows of this lane's pieces, looked up before the pieces are asked for (both operands' pieces lie alike if BP == BQ)
+    int row_p[kPCols ? NP : 1], row_q[kPCols && BP != BQ ? NQ : 1];
+    auto look_up = [&](int step) {
+        asm volatile("" : "+v"(now_lane));
+        if constexpr (kPCols) {
 #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const T* p;
-            int have;  // elements of the chunk that exist (DMA: all or none)
+            for (int n = 0; n < NP; ++n) row_p[n] = row_of(step * BC + col_row(n, NP, BP));
+            if constexpr (BP != BQ)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) row_q[n] = row_of(step * BC + col_row(n, NQ, BQ));
+        }
+    };
+    // piece n (P's, then Q's) of a step; DMA: into LDS, otherwise into hold_*
+    auto load = [&](int n, int step, int stage) {
+        const int c0 = step * BC;
+        const T* p;
+        int have;  // elements of the chunk that exist (DMA: all or none)
+        unsigned to = lds_address(smem + stage * kStage);
+        if (n < NP) {
             if constexpr (kPCols) {
-                const int r = row_of(c0 + c_p[n]);
-                have = r >= 0 ? (DMA ? 8 : n_p - col_p[n]) : 0;
-                p = P + (int64_t)r * a.ld_p + col_p[n];
+                const int c = col_row(n, NP, BP);
+                int col = p0 + 8 * ((((wave * NP + n) * 64 + now_lane) % (BP / 8)) ^ (spread<BP>(c) >> 4));
+                have = row_p[n] >= 0 ? (DMA ? 8 : n_p - col) : 0;
+                if (DMA && col >= n_p) col = 0;  // columns past the end: any, not stored
+                p = P + (int64_t)row_p[n] * a.ld_p + col;
             } else {
-                have = n_c - c0 - c_p[n];
+                have = n_c - c0 - c_p;
                 p = src_p[n] + c0;
             }
-            if (DMA) glds16(have > 0 ? p : zeros, __builtin_amdgcn_readfirstlane(to_p + n * 1024));
-            else hold_p[n] = load_piece(p, have);
-        }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const T* q;
-            int have;
+            to += (wave * NP + n) * 1024;
+        } else {
+            const int m = n - NP;
             if constexpr (kQCols) {
-                const int c = c0 + c_q[n], r = PRODUCT == kGradWeight ? row_of(c) : c < n_c ? c : -1;
-                have = r >= 0 ? (DMA ? 8 : n_q - col_q[n]) : 0;
-                q = Q + (int64_t)r * a.ld_q + col_q[n];
+                const int c = col_row(m, NQ, BQ);
+                int r, col = q0 + 8 * ((((wave * NQ + m) * 64 + now_lane) % (BQ / 8)) ^ (spread<BQ>(c) >> 4));
+                if constexpr (PRODUCT == kGradWeight) r = BP != BQ ? row_q[BP != BQ ? m : 0] : row_p[m];
+                else r = c0 + c < n_c ? c0 + c : -1;
+                have = r >= 0 ? (DMA ? 8 : n_q - col) : 0;
+                if (DMA && col >= n_q) col = 0;
+                p = Q + (int64_t)r * a.ld_q + col;
             } else {
-                have = n_c - c0 - c_q[n];
-                q = src_q[n] + c0;
+                have = n_c - c0 - c_q;
+                p = src_q[m] + c0;
             }
-            if (DMA) glds16(have > 0 ? q : zeros, __builtin_amdgcn_readfirstlane(to_q + n * 1024));
-            else hold_q[n] = load_piece(q, have);
+            to += kPBytes * F::kPlanes + (wave * NQ + m) * 1024;
         }
+        if (DMA) glds16(have > 0 ? p : zeros, __builtin_amdgcn_readfirstlane(to));
+        else if (n < NP) hold_p[DMA || n >= NP ? 0 : n] = load_piece(p, have);
+        else hold_q[DMA || n < NP ? 0 : n - NP] = load_piece(p, have);
+    };
+    auto load_all = [&](int step, int stage) {
+        look_up(step);
+#pragma unroll
+        for (int n = 0; n < NP + NQ; ++n) load(n, step, stage);
     };
     auto store = [&](int stage) {
         char* s = smem + stage * kStage;
@@ -365,96 +408,161 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 
     // ---- fragments
     const int pw = BP / WP * (wave % WP), qw = BQ / WQ * (wave / WP), fr = lane & 15, kg = lane >> 4;
-    auto frag = [&](auto cols, auto width, const char* tile, int first, int i, int kk) -> V {
-        constexpr bool C = decltype(cols)::value;
+    // byte offset of fragment 0 in its tile; fragment i: "rows" + 16 i rows, "columns" ^ 32 i (no carry: 16 x fragments divides a
+    // wave's first column).  The second 32 contraction elements: "rows" ^ 64, "columns" + 32 rows.
+    auto frag_at = [&](auto cols, auto width, int first) {
         constexpr int B = decltype(width)::value;
-        if constexpr (C) {
-            const int c = 32 * kk + 8 * kg + (fr >> 2);  // rows c and c + 4
-            return columns_frag<V>(tile + c * (2 * B) + ((2 * (first + 16 * i)) ^ spread<B>(8 * kg + (fr >> 2))) + 8 * (fr & 3), 4 * 2 * B);
+        if constexpr (decltype(cols)::value) {
+            const int c = 8 * kg + (fr >> 2);  // rows c and c + 4
+            return c * (2 * B) + ((2 * first) ^ spread<B>(c)) + 8 * (fr & 3);
         } else {
-            const int r = first + 16 * i + fr;
-            return *reinterpret_cast<const V*>(tile + r * (2 * BC) + (((4 * kk + kg) ^ turn<BC>(fr)) << 4));
+            return (first + fr) * (2 * BC) + ((kg ^ turn<BC>(fr)) << 4);
         }
     };
-    f32x4 acc[FP][FQ] = {}, accb[FP] = {};
-    // db: the sum of dy's columns as one more product, by ones; a long plain sum loses more than a product's, so every kSegment rows
-    // the running sum goes into a second one (rounding of n terms ~ sqrt(n / 1024) + sqrt(256) instead of sqrt(n / 4) steps)
-    float sumb[FP] = {};
+    auto frag = [&](auto cols, auto width, const char* tile, int at, int i, int kk) -> V {
+        constexpr int B = decltype(width)::value;
+        if constexpr (decltype(cols)::value) return columns_frag<V>(tile + (at ^ (32 * i)) + kk * 32 * (2 * B), 4 * 2 * B);
+        else return *reinterpret_cast<const V*>(tile + (at ^ (64 * kk)) + 16 * i * (2 * BC));
+    };
+    int at_p = frag_at(std::integral_constant<bool, kPCols>(), std::integral_constant<int, BP>(), pw);
+    int at_q = frag_at(std::integral_constant<bool, kQCols>(), std::integral_constant<int, BQ>(), qw);
+    f32x4 acc[FP][FQ] = {};
+    // db: this lane's share of the sums of dy's columns.  fp32 results: a plain sum loses more than torch's pairwise one, so every
+    // kSegment rows the running sum goes into a second one
+    float accb[FP] = {}, sumb[FP] = {};
     const bool sum_bias = PRODUCT == kGradWeight && a.dbias && q0 == 0 && qw == 0;
-    V ones;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ones[i] = (typename F::E)1.0f;
-    auto multiply = [&](const char* tp) {
-        const char* tq = tp + F::kPlanes * kPBytes;
-#pragma unroll
-        for (int kk = 0; kk < BC / 32; ++kk) {
-            V fq[F::kPlanes][FQ];
-#pragma unroll
-            for (int l = 0; l < F::kPlanes; ++l)
-#pragma unroll
-                for (int j = 0; j < FQ; ++j)
-                    fq[l][j] = frag(std::integral_constant<bool, kQCols>(), std::integral_constant<int, BQ>(), tq + l * kQBytes, qw, j, kk);
-#pragma unroll
-            for (int l = F::kPlanes - 1; l >= 0; --l) {
-                V fp[FP];
-#pragma unroll
-                for (int i = 0; i < FP; ++i)
-                    fp[i] = frag(std::integral_constant<bool, kPCols>(), std::integral_constant<int, BP>(), tp + l * kPBytes, pw, i, kk);
-#pragma unroll
-                for (int m = F::kPlanes - 1 - l; m >= 0; --m)
-#pragma unroll
-                    for (int i = 0; i < FP; ++i)
-#pragma unroll
-                        for (int j = 0; j < FQ; ++j) acc[i][j] = F::mfma(fq[m][j], fp[i], acc[i][j]);
-                if (sum_bias)
-#pragma unroll
-                    for (int i = 0; i < FP; ++i) accb[i] = F::mfma(ones, fp[i], accb[i]);
-            }
-        }
+    auto p_frag = [&](const char* stage, int l, int i, int kk) {
+        return frag(std::integral_constant<bool, kPCols>(), std::integral_constant<int, BP>(), stage + l * kPBytes, at_p, i, kk);
     };
-
+    auto q_frag = [&](const char* stage, int l, int j, int kk) {
+        return frag(std::integral_constant<bool, kQCols>(), std::integral_constant<int, BQ>(), stage + F::kPlanes * kPBytes + l * kQBytes, at_q, j, kk);
+    };
     if (steps > 0) {
         fetch_segment(0);
         if (PRODUCT == kGradWeight && a.order) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            wait_loads<0>();
             __syncthreads();
         }
-        load(0, 0);
-        if (!DMA && !kWide) store(0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        barrier_lds_only();
     }
-    for (int s = 0; s < steps; ++s) {
-        if (s % (kSegment / BC) == 0) {
-            fetch_segment(s / (kSegment / BC) + 1);  // the segment before s's is no longer read
-            if (sum_bias)
+    if constexpr (DMA) {
+        // Two halves of 32 contraction elements a step.  While the matrix instructions of one half run, the fragments of the next are
+        // read: the second half's during the first; the barrier between them says that everybody has read this stage and that the
+        // next one has arrived; during the second half the next step's first fragments are read and the step after it is asked for,
+        // into the stage just read.  A P fragment's register takes its successor as soon as its products are issued; the last two
+        // and Q's have two sets, so that all reads of a half are issued two groups before they are waited for.
+        static_assert(BC == 64 && STAGES == 2 && FP >= 4 && FQ <= FP, "two halves, two stages");
+        constexpr int NL = NP + NQ, NT2 = FP - 2;
+        V fp[NT2], tail[2][2], fq[2][FQ];
+        auto read_group = [&](int g, int half, int stage) {  // of group g: the reads for `half` of `stage`
+            const char* at = smem + stage * kStage;
+            if (g < 2) tail[half][g] = p_frag(at, 0, NT2 + g, half);
+            if (g < FQ) fq[half][g] = q_frag(at, 0, g, half);
+            if (g >= 1 && g - 1 < NT2) fp[g - 1] = p_frag(at, 0, g - 1, half);
+        };
+        auto multiply = [&](auto with_bias, int i, int half) {
+            const V p = i < NT2 ? fp[i < NT2 ? i : 0] : tail[half][i < NT2 ? 0 : i - NT2];
 #pragma unroll
-                for (int i = 0; i < FP; ++i) sumb[i] += accb[i][0], accb[i] = f32x4{};
+            for (int j = 0; j < FQ; ++j) acc[i][j] = F::mfma(fq[half][j], p, acc[i][j]);
+            if (decltype(with_bias)::value) accb[i] = add_elements(p, accb[i]);
+        };
+        if (steps > 0) {
+            load_all(0, 0);
+            load_all(1, 1);
+            wait_loads<NL>();
+            barrier_lds_only();
+#pragma unroll
+            for (int g = 0; g < FP; ++g) read_group(g, 0, 0);
         }
-        if (kWide) {
-            store(0);
+        auto all_steps = [&](auto with_bias) {
+            for (int s = 0; s < steps; ++s) {
+                const int now = s & 1;
+                if (s % (kSegment / BC) == 0) fetch_segment(s / (kSegment / BC) + 1);  // the segment before s's is no longer read
+                asm volatile("" : "+v"(at_p), "+v"(at_q));  // as now_lane: the fragments' offsets are made where they are used
+#pragma unroll
+                for (int g = 0; g < FP; ++g) {
+                    multiply(with_bias, g, 0);
+                    read_group(g, 1, now);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                wait_loads<0>();
+                barrier_lds_only();
+                look_up(s + 2);
+#pragma unroll
+                for (int g = 0; g < FP; ++g) {
+                    multiply(with_bias, g, 1);
+                    read_group(g, 0, now ^ 1);
+#pragma unroll
+                    for (int n = g * NL / FP; n < (g + 1) * NL / FP; ++n) load(n, s + 2, now);  // past the last step: zeros, nobody reads them
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        };
+        if (PRODUCT == kGradWeight && sum_bias) all_steps(std::integral_constant<bool, PRODUCT == kGradWeight>());
+        else all_steps(std::false_type());
+        wait_loads<0>();  // no load may outlive its workgroup's LDS
+    } else {
+        // through registers: all of Q's fragments against one of P's after the other, which are read two ahead
+        auto multiply = [&](const char* at) {
+            constexpr int KK = BC / 32, NI = KK * F::kPlanes * FP;  // P fragments of the stage: [kk][plane][i]
+            V fq[F::kPlanes][FQ], fp[3];
+            auto read_p = [&](int x) { return p_frag(at, F::kPlanes - 1 - x / FP % F::kPlanes, x % FP, x / (F::kPlanes * FP)); };
+            fp[0] = read_p(0);
+            fp[1] = read_p(1);
+#pragma unroll
+            for (int x = 0; x < NI; ++x) {
+                const int i = x % FP, l = F::kPlanes - 1 - x / FP % F::kPlanes;
+                if (x % (F::kPlanes * FP) == 0)
+#pragma unroll
+                    for (int m = 0; m < F::kPlanes; ++m)
+#pragma unroll
+                        for (int j = 0; j < FQ; ++j) fq[m][j] = q_frag(at, m, j, x / (F::kPlanes * FP));
+                if (x + 2 < NI) fp[(x + 2) % 3] = read_p(x + 2);
+#pragma unroll
+                for (int m = F::kPlanes - 1 - l; m >= 0; --m)
+#pragma unroll
+                    for (int j = 0; j < FQ; ++j) acc[i][j] = F::mfma(fq[m][j], fp[x % 3], acc[i][j]);
+                if (sum_bias) accb[i] = add_elements(fp[x % 3], accb[i]);
+            }
+        };
+        if (steps > 0) {
+            load_all(0, 0);
+            if (!kAhead) {
+                store(0);
+                barrier_lds_only();
+            }
+        }
+        for (int s = 0; s < steps; ++s) {
+            const int now = kAhead ? 0 : s & 1;
+            if (s % (kSegment / BC) == 0) {
+                fetch_segment(s / (kSegment / BC) + 1);  // the segment before s's is no longer read
+                if (kWide && sum_bias)
+#pragma unroll
+                    for (int i = 0; i < FP; ++i) sumb[i] += accb[i], accb[i] = 0.0f;
+            }
+            if (kAhead) {
+                store(0);
+                barrier_lds_only();
+            }
+            if (s + 1 < steps) load_all(s + 1, 0);
+            multiply(smem + now * kStage);
+            if (!kAhead && s + 1 < steps) store(now ^ 1);
+            wait_loads<0>();
             barrier_lds_only();
         }
-        if (s + 1 < steps) load(s + 1, (s + 1) & 1);
-        multiply(smem + (kWide ? 0 : s & 1) * kStage);
-        if (!DMA && !kWide && s + 1 < steps) store((s + 1) & 1);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        barrier_lds_only();
     }
     if constexpr (kWide) {
         // an infinity among the operands: the sums again, element by element from memory (rare, and as slow as that sounds)
         if (__syncthreads_or(infinite)) {
             for (int i = 0; i < FP; ++i) {
                 const int p = pw + 16 * i + fr, row = kPCols ? 0 : rows_lds[p];
-                sumb[i] = 0.0f;
-                accb[i] = f32x4{};
+                sumb[i] = accb[i] = 0.0f;
                 for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{};
                 if (kPCols ? p0 + p >= n_p : row < 0) continue;
                 for (int c = 0; c < n_c; ++c) {
                     const int r = kPCols ? (a.order ? a.order[tl.first + c] : tl.first + c) : row;
                     if ((unsigned)r >= (unsigned)rows) continue;
                     const float x = P[(int64_t)r * a.ld_p + (kPCols ? p0 + p : c)];
-                    sumb[i] += x;
+                    sumb[i] += kg == 0 ? x : 0.0f;
                     for (int j = 0; j < FQ; ++j)
                         for (int e = 0; e < 4; ++e) {
                             const int q = q0 + qw + 16 * j + 4 * kg + e;
@@ -508,8 +616,11 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
                     if (q + e < n_q) static_cast<T*>(a.out)[at + q + e] = (T)v[e];
             }
         }
-        if (sum_bias && lane < 16) {
-            const float v = sumb[i] + accb[i][0];
+        if (sum_bias) {
+            float v = sumb[i] + accb[i];  // of the rows 8 kg .. 8 kg + 7 of every 32
+            v += __shfl_xor(v, 16);
+            v += __shfl_xor(v, 32);
+            if (kg != 0) continue;
             if (a.chunk_rows) a.part[(int64_t)a.chunks * a.n_out * a.n_in + (int64_t)run * a.n_out + p0 + p] = v;
             else static_cast<T*>(a.dbias)[(int64_t)tl.g * a.n_out + p0 + p] = (T)v;
         }
@@ -561,10 +672,10 @@ int check_grid(int64_t blocks) {
     return MCMC_OK;
 }
 
-template <typename T, int PRODUCT, int BP, int BQ, int WP, int WQ, bool DMA>
+template <typename T, int PRODUCT, int BP, int BQ, int WP, int WQ, bool DMA, int BC, int STAGES>
 int launch_tile(unsigned blocks, const Args& a, hipStream_t s) {
-    const size_t lds = (sizeof(T) == 4 ? 3 * 64 : 2 * 128) * (size_t)(BP + BQ) + (PRODUCT == kGradWeight ? 2 * kSegment : BP) * sizeof(int);
-    const auto kern = grouped_tile_kernel<T, PRODUCT, BP, BQ, WP, WQ, DMA>;
+    const size_t lds = (size_t)STAGES * (BP + BQ) * BC * 2 * Frag<T>::kPlanes + (PRODUCT == kGradWeight ? 2 * kSegment : BP) * sizeof(int);
+    const auto kern = grouped_tile_kernel<T, PRODUCT, BP, BQ, WP, WQ, DMA, BC, STAGES>;
     if (int rc = ensure_dyn_lds((const void*)kern, lds, "grouped_tile_kernel")) return rc;
     kern<<<blocks, 64 * WP * WQ, lds, s>>>(a);
     return check_launch("grouped_tile_kernel");
@@ -579,10 +690,12 @@ bool whole_chunks(int product, const Args& a) {
 template <typename T, int PRODUCT>
 int launch_product(const Args& a, Shape sh, bool dma, unsigned blocks, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
-        if (sh.bp == 256) return launch_tile<T, PRODUCT, 256, 256, 2, 4, true>(blocks, a, s);
-        if (dma) return launch_tile<T, PRODUCT, 128, 128, 2, 2, true>(blocks, a, s);
+        if (sh.bp == 256) return launch_tile<T, PRODUCT, 256, 256, 2, 4, true, 64, 2>(blocks, a, s);
+        if (dma) return launch_tile<T, PRODUCT, 128, 128, 2, 2, true, 64, 2>(blocks, a, s);
+        return launch_tile<T, PRODUCT, 128, 128, 2, 2, false, 32, 2>(blocks, a, s);
+    } else {
+        return launch_tile<T, PRODUCT, 128, 128, 2, 2, false, 32, 1>(blocks, a, s);
     }
-    return launch_tile<T, PRODUCT, 128, 128, 2, 2, false>(blocks, a, s);
 }
 
 template <typename T>
