@@ -23,7 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .engine import Engine, _p, _require_gpu, _stream
+from .engine import Engine
 
 _DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 _ACT = {None: _lib.ACT_NONE, "none": _lib.ACT_NONE, "elu": _lib.ACT_ELU}
@@ -33,11 +33,15 @@ _MAX_DIM = 1 << 30       # MCMC_GROUPED_MAX_ROWS, MCMC_GROUPED_MAX_DIM
 _ENGINES = {}
 
 
+# The calls on small batches last as long as their Python: pointers and the stream go to the library as plain integers (ctypes
+# converts those fastest), sizes are taken once, and what needs no gradient does not pass through autograd.
 def _engine(t: torch.Tensor, what: str, **others: Optional[torch.Tensor]) -> Engine:
     """The engine of t's device; every other tensor has to live there too."""
-    dev = _require_gpu(t, what)
-    for name, o in others.items():
-        if o is not None and _require_gpu(o, name) != dev:
+    dev = t.get_device()
+    for name, o in ((what, t), *others.items()):
+        if o is not None and o.get_device() != dev or dev < 0:
+            if not o.is_cuda:
+                raise RuntimeError(f"{name} must live on a HIP device (got {o.device}); mcmc_amd has no CPU path")
             raise ValueError(f"{name} lives on {o.device}, {what} on {t.device}")
     eng = _ENGINES.get(dev)
     if eng is None:
@@ -45,8 +49,19 @@ def _engine(t: torch.Tensor, what: str, **others: Optional[torch.Tensor]) -> Eng
     return eng
 
 
+_HERE = nullcontext()
+
+
 def _on(eng: Engine):
-    return nullcontext() if torch.cuda.current_device() == eng.device.index else torch.cuda.device(eng.device)
+    return _HERE if torch.cuda.current_device() == eng.device.index else torch.cuda.device(eng.device)
+
+
+def _stream(eng: Engine) -> int:
+    return torch._C._cuda_getCurrentRawStream(eng.device.index)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -64,6 +79,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """[..., width] as [rows, width] (empty tensors included)."""
     return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+
+
+def _wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 class RowGroups(NamedTuple):
@@ -95,47 +114,47 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
         order = torch.empty(rows, dtype=torch.int32, device=ids.device)
         offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=ids.device)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=ids.device) if ws_bytes else None
-        _lib.check(eng.lib.mcmc_group_rows(eng.ctx.handle, _p(ids), ids.element_size(), rows, n_groups, _p(order), _p(offsets), _p(ws), _stream()),
-                   "mcmc_group_rows")
+        _lib.check(eng.lib.mcmc_group_rows(eng.ctx.handle, ids.data_ptr(), ids.element_size(), rows, n_groups, order.data_ptr(), offsets.data_ptr(),
+                                           _ptr(ws), _stream(eng)), "mcmc_group_rows")
     return RowGroups(order, offsets)
 
 
 # ---- grouped_linear ---------------------------------------------------------------------------------------------------------
 def _forward(eng: Engine, x, weight, bias, order, offsets):
-    G, N, K = weight.shape
-    y = torch.empty(x.shape[0], N, dtype=x.dtype, device=x.device)
-    _lib.check(eng.lib.mcmc_grouped_linear_forward(eng.ctx.handle, _DT[x.dtype], _p(x), x.stride(0), x.shape[0], _p(order), _p(offsets), G, K, N,
-                                                   _p(weight), _p(bias), _p(y), _stream()), "mcmc_grouped_linear_forward")
+    (R, K), (G, N, _) = x.shape, weight.shape
+    y = torch.empty((R, N), dtype=x.dtype, device=x.device)
+    _lib.check(eng.lib.mcmc_grouped_linear_forward(eng.ctx.handle, _DT[x.dtype], x.data_ptr(), x.stride(0), R, _ptr(order), offsets.data_ptr(), G, K, N,
+                                                   weight.data_ptr(), _ptr(bias), y.data_ptr(), _stream(eng)), "mcmc_grouped_linear_forward")
     return y
 
 
 def _grad_input(eng: Engine, dy, weight, order, offsets):
-    G, N, K = weight.shape
-    dx = torch.empty(dy.shape[0], K, dtype=dy.dtype, device=dy.device)
-    _lib.check(eng.lib.mcmc_grouped_linear_grad_input(eng.ctx.handle, _DT[dy.dtype], _p(dy), dy.stride(0), dy.shape[0], _p(order), _p(offsets), G, K, N,
-                                                      _p(weight), _p(dx), _stream()), "mcmc_grouped_linear_grad_input")
+    R, (G, N, K) = dy.shape[0], weight.shape
+    dx = torch.empty((R, K), dtype=dy.dtype, device=dy.device)
+    _lib.check(eng.lib.mcmc_grouped_linear_grad_input(eng.ctx.handle, _DT[dy.dtype], dy.data_ptr(), dy.stride(0), R, _ptr(order), offsets.data_ptr(), G, K, N,
+                                                      weight.data_ptr(), dx.data_ptr(), _stream(eng)), "mcmc_grouped_linear_grad_input")
     return dx
 
 
 def _grad_weight(eng: Engine, dy, x, order, offsets, G: int, want_bias: bool):
-    R, N, K = x.shape[0], dy.shape[1], x.shape[1]
-    ws_bytes = _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(_DT[x.dtype], R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    dw = torch.empty(G, N, K, dtype=x.dtype, device=x.device)
-    db = torch.empty(G, N, dtype=x.dtype, device=x.device) if want_bias else None
-    _lib.check(eng.lib.mcmc_grouped_linear_grad_weight(eng.ctx.handle, _DT[x.dtype], _p(dy), dy.stride(0), _p(x), x.stride(0), R, _p(order), _p(offsets),
-                                                       G, K, N, _p(dw), _p(db), _p(ws), _stream()), "mcmc_grouped_linear_grad_weight")
+    (R, K), N, dt, dev = x.shape, dy.shape[1], _DT[x.dtype], x.device
+    ws_bytes = _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(dt, R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    dw = torch.empty((G, N, K), dtype=x.dtype, device=dev)
+    db = torch.empty((G, N), dtype=x.dtype, device=dev) if want_bias else None
+    _lib.check(eng.lib.mcmc_grouped_linear_grad_weight(eng.ctx.handle, dt, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), R, _ptr(order),
+                                                       offsets.data_ptr(), G, K, N, dw.data_ptr(), _ptr(db), _ptr(ws), _stream(eng)),
+               "mcmc_grouped_linear_grad_weight")
     return dw, db
 
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, order, offsets):
-        eng = _engine(x, "x", weight=weight, bias=bias, order=order, offsets=offsets)
+    def forward(ctx, eng, x, weight, bias, order, offsets):
         with _on(eng):
             x, weight = _rows(x), weight.contiguous()
             y = _forward(eng, x, weight, None if bias is None else bias.contiguous(), order, offsets)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_x, need_w, need_b = ctx.needs_input_grad[1:4]
         ctx.eng, ctx.shape = eng, weight.shape
         # what each gradient reads: dx the weights, dW the inputs
         ctx.save_for_backward(x if need_w or need_b else None, weight if need_x else None, order, offsets)
@@ -146,7 +165,7 @@ class _GroupedLinear(torch.autograd.Function):
     def backward(ctx, dy):
         eng = ctx.eng
         x, weight, order, offsets = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_x, need_w, need_b = ctx.needs_input_grad[1:4]
         dx = dw = db = None
         with _on(eng):
             dy = _rows(dy)
@@ -154,7 +173,7 @@ class _GroupedLinear(torch.autograd.Function):
                 dx = _grad_input(eng, dy, weight, order, offsets)
             if need_w or need_b:
                 dw, db = _grad_weight(eng, dy, x, order, offsets, ctx.shape[0], need_b)
-        return dx, dw if need_w else None, db, None, None
+        return None, dx, dw if need_w else None, db, None, None
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -163,54 +182,65 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
     x [rows, in]; weight [n_groups, out, in]; bias [n_groups, out]; all of one type (float32, bfloat16 or float16; sums are
     kept in 32 bits and rounded once).  Differentiable in x, weight and bias; a group without rows gets zero gradients."""
     order, offsets = groups
-    if x.dim() != 2 or weight.dim() != 3 or (bias is not None and bias.dim() != 2):
-        raise ValueError(f"x must be [rows, in], weight [groups, out, in], bias [groups, out]; got {tuple(x.shape)}, {tuple(weight.shape)}"
+    xs, ws = x.shape, weight.shape
+    if len(xs) != 2 or len(ws) != 3 or (bias is not None and bias.dim() != 2):
+        raise ValueError(f"x must be [rows, in], weight [groups, out, in], bias [groups, out]; got {tuple(xs)}, {tuple(ws)}"
                          + ("" if bias is None else f", {tuple(bias.shape)}"))
     _dtype(x, "x")
-    G, N, K = weight.shape
-    if min(G, N, K) < 1 or max(G, N, K, x.shape[0]) > _MAX_DIM:
-        raise ValueError(f"every size of weight must be in [1, 2^30] and rows at most 2^30, got {tuple(weight.shape)} and {x.shape[0]} rows")
-    if x.shape[1] != K:
-        raise ValueError(f"Expected {K} input features, got {x.shape[1]}")
+    (R, K), (G, N, weight_in) = xs, ws
+    if min(G, N, weight_in) < 1 or max(G, N, weight_in, R) > _MAX_DIM:
+        raise ValueError(f"every size of weight must be in [1, 2^30] and rows at most 2^30, got {tuple(ws)} and {R} rows")
+    if K != weight_in:
+        raise ValueError(f"Expected {weight_in} input features, got {K}")
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise ValueError(f"x, weight and bias must have one type, got {x.dtype}, {weight.dtype}" + ("" if bias is None else f", {bias.dtype}"))
-    if bias is not None and tuple(bias.shape) != (G, N):
+    if bias is not None and bias.shape != (G, N):
         raise ValueError(f"bias must be {(G, N)}, got {tuple(bias.shape)}")
-    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (G + 1,) or not offsets.is_contiguous():
+    if offsets.dtype != torch.int32 or offsets.shape != (G + 1,) or not offsets.is_contiguous():
         raise ValueError(f"groups.offsets must be a contiguous int32 [{G + 1}] tensor (n_groups + 1), got {offsets.dtype} {tuple(offsets.shape)}")
-    if order is not None and (order.dtype != torch.int32 or tuple(order.shape) != (x.shape[0],) or not order.is_contiguous()):
-        raise ValueError(f"groups.order must be None or a contiguous int32 [{x.shape[0]}] tensor (rows), got {order.dtype} {tuple(order.shape)}")
-    return _GroupedLinear.apply(x, weight, bias, order, offsets)
+    if order is not None and (order.dtype != torch.int32 or order.shape != (R,) or not order.is_contiguous()):
+        raise ValueError(f"groups.order must be None or a contiguous int32 [{R}] tensor (rows), got {order.dtype} {tuple(order.shape)}")
+    eng = _engine(x, "x", weight=weight, bias=bias, order=order, offsets=offsets)
+    if _wants_grad(x, weight, bias):
+        return _GroupedLinear.apply(eng, x, weight, bias, order, offsets)
+    with _on(eng):
+        return _forward(eng, _rows(x), weight.contiguous(), None if bias is None else bias.contiguous(), order, offsets)
 
 
 # ---- philox_dropout ---------------------------------------------------------------------------------------------------------
+def _dropout(eng: Engine, x, args):
+    """y [rows, width] and the 2-D x it was made from."""
+    p, seed, seed_dev, act, pair, row_begin, elem_begin = args
+    x = _rows(_flat(x))
+    R, W = x.shape
+    y = torch.empty((R, W), dtype=x.dtype, device=x.device)
+    _lib.check(eng.lib.mcmc_dropout_forward(eng.ctx.handle, _DT[x.dtype], act, x.data_ptr(), x.stride(0), R, W, seed, _ptr(seed_dev), p, pair, row_begin,
+                                            elem_begin, y.data_ptr(), W, _stream(eng)), "mcmc_dropout_forward")
+    return y, x
+
+
 class _PhiloxDropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, p, seed, seed_dev, act, pair, row_begin, elem_begin):
-        eng = _engine(x, "x", seed=seed_dev)
-        dt = _DT[x.dtype]
+    def forward(ctx, eng, x, seed_dev, args):
         with _on(eng):
-            x2 = _rows(_flat(x))
-            y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
-            _lib.check(eng.lib.mcmc_dropout_forward(eng.ctx.handle, dt, act, _p(x2), x2.stride(0), x2.shape[0], x2.shape[1], seed, _p(seed_dev), p, pair,
-                                                    row_begin, elem_begin, _p(y), x2.shape[1], _stream()), "mcmc_dropout_forward")
-        if ctx.needs_input_grad[0]:
-            ctx.eng, ctx.args, ctx.shape = eng, (p, seed, act, pair, row_begin, elem_begin), x.shape
-            ctx.save_for_backward(x2 if act != _lib.ACT_NONE else None, seed_dev)
+            y, x2 = _dropout(eng, x, args)
+        ctx.eng, ctx.args, ctx.shape = eng, args, x.shape
+        ctx.save_for_backward(x2 if args[3] != _lib.ACT_NONE else None, seed_dev)
         return y.view(x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        eng, (p, seed, act, pair, row_begin, elem_begin) = ctx.eng, ctx.args
-        x2, seed_dev = ctx.saved_tensors
+        eng, (p, seed, _, act, pair, row_begin, elem_begin) = ctx.eng, ctx.args
+        x, seed_dev = ctx.saved_tensors
         with _on(eng):
-            dy2 = _rows(_flat(dy))
-            dx = torch.empty(dy2.shape, dtype=dy.dtype, device=dy.device)
-            _lib.check(eng.lib.mcmc_dropout_backward(eng.ctx.handle, _DT[dy.dtype], act, _p(dy2), dy2.stride(0), _p(x2), 0 if x2 is None else x2.stride(0),
-                                                     dy2.shape[0], dy2.shape[1], seed, _p(seed_dev), p, pair, row_begin, elem_begin, _p(dx), dy2.shape[1],
-                                                     _stream()), "mcmc_dropout_backward")
-        return dx.view(ctx.shape), None, None, None, None, None, None, None
+            dy = _rows(_flat(dy))
+            R, W = dy.shape
+            dx = torch.empty((R, W), dtype=dy.dtype, device=dy.device)
+            _lib.check(eng.lib.mcmc_dropout_backward(eng.ctx.handle, _DT[dy.dtype], act, dy.data_ptr(), dy.stride(0), _ptr(x), 0 if x is None else x.stride(0),
+                                                     R, W, seed, _ptr(seed_dev), p, pair, row_begin, elem_begin, dx.data_ptr(), W, _stream(eng)),
+                       "mcmc_dropout_backward")
+        return None, dx.view(ctx.shape), None, None
 
 
 def philox_dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], *, activation: Optional[str] = None, pair: int = 0,
@@ -239,4 +269,9 @@ def philox_dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], *,
         if seed.dtype != torch.int64 or seed.numel() != 1:
             raise ValueError(f"a seed tensor must hold one int64, got {seed.dtype} {tuple(seed.shape)}")
         seed, seed_dev = 0, seed
-    return _PhiloxDropout.apply(x, float(p), int(seed) & _U64, seed_dev, _ACT[activation], int(pair), int(row_begin), int(elem_begin))
+    eng = _engine(x, "x", seed=seed_dev)
+    args = (float(p), int(seed) & _U64, seed_dev, _ACT[activation], int(pair), int(row_begin), int(elem_begin))
+    if _wants_grad(x):
+        return _PhiloxDropout.apply(eng, x, seed_dev, args)
+    with _on(eng):
+        return _dropout(eng, x, args)[0].view(x.shape)
