@@ -53,7 +53,7 @@ _HERE = nullcontext()
 
 
 def _on(eng: Engine):
-    return _HERE if torch.cuda.current_device() == eng.device.index else torch.cuda.device(eng.device)
+    return _HERE if torch._C._cuda_getDevice() == eng.device.index else torch.cuda.device(eng.device)
 
 
 def _stream(eng: Engine) -> int:
@@ -79,6 +79,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """[..., width] as [rows, width] (empty tensors included)."""
     return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+
+
+def _once(backward):
+    """Gradients of gradients are refused like once_differentiable does it, but its bookkeeping (20 us a call) is paid only by a
+    backward pass that records a graph."""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, dy):
+        return recorded(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
+    return run
 
 
 def _wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
@@ -161,7 +171,7 @@ class _GroupedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         eng = ctx.eng
         x, weight, order, offsets = ctx.saved_tensors
@@ -224,23 +234,26 @@ class _PhiloxDropout(torch.autograd.Function):
     def forward(ctx, eng, x, seed_dev, args):
         with _on(eng):
             y, x2 = _dropout(eng, x, args)
-        ctx.eng, ctx.args, ctx.shape = eng, args, x.shape
+        ctx.eng, ctx.args, ctx.sizes = eng, args, x2.shape
         ctx.save_for_backward(x2 if args[3] != _lib.ACT_NONE else None, seed_dev)
         return y.view(x.shape)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         eng, (p, seed, _, act, pair, row_begin, elem_begin) = ctx.eng, ctx.args
         x, seed_dev = ctx.saved_tensors
+        R, W = ctx.sizes
         with _on(eng):
-            dy = _rows(_flat(dy))
-            R, W = dy.shape
-            dx = torch.empty((R, W), dtype=dy.dtype, device=dy.device)
-            _lib.check(eng.lib.mcmc_dropout_backward(eng.ctx.handle, _DT[dy.dtype], act, dy.data_ptr(), dy.stride(0), _ptr(x), 0 if x is None else x.stride(0),
-                                                     R, W, seed, _ptr(seed_dev), p, pair, row_begin, elem_begin, dx.data_ptr(), W, _stream(eng)),
+            dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
+            ld = W
+            if not dy.is_contiguous():
+                dy = _rows(_flat(dy))
+                ld = dy.stride(0)
+            _lib.check(eng.lib.mcmc_dropout_backward(eng.ctx.handle, _DT[dy.dtype], act, dy.data_ptr(), ld, _ptr(x), 0 if x is None else x.stride(0), R, W,
+                                                     seed, _ptr(seed_dev), p, pair, row_begin, elem_begin, dx.data_ptr(), W, _stream(eng)),
                        "mcmc_dropout_backward")
-        return None, dx.view(ctx.shape), None, None
+        return None, dx, None, None
 
 
 def philox_dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], *, activation: Optional[str] = None, pair: int = 0,

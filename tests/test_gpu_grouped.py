@@ -572,3 +572,14 @@ def test_fp32_infinities_and_the_whole_range(K, N):
         ref, mag = linear_reference(x2, w2, b * 0, dy.clamp(-3, 3), ids)
         for n in ("y", "dx"):
             check(got[n], ref[n], mag[n] * U, n)
+
+
+def test_gradients_of_gradients_are_refused():
+    x, w, b, dy, groups, ids = linear_case(20, 2, 8, 8, FP32, 600)
+    for f in (lambda t: grouped_linear(t, w, groups, b), lambda t: philox_dropout(t, 0.1, 5, activation="elu")):
+        t = x.detach().requires_grad_()
+        first, = torch.autograd.grad(f(t).square().sum(), t, create_graph=True)
+        plain, = torch.autograd.grad(f(t).square().sum(), t)
+        assert torch.equal(first.detach(), plain)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
