@@ -3,13 +3,15 @@
 //   order   = the rows 0..R-1 sorted stably by key, key(r) = ids[r] if 0 <= ids[r] < G, else G (no group: last)
 //   offsets = offsets[g] = number of rows with key < g, g = 0..G
 //
-// A stable counting sort.  The rows are cut into chunks, one wave each; a wave walks its chunk 64 rows at a time and finds the
-// lanes that hold the same key by one ballot per key bit (match_key), so the rank of a row among its equals is a popcount:
-// no atomics, the result is a function of the ids alone.
+// A stable counting sort.  The rows are cut into chunks, one wave each, with counters of their own in LDS; a wave walks its chunk 64
+// rows at a time and finds the lanes that hold the same key by one ballot per key bit (match_key), so the rank of a row among its
+// equals is a popcount.  Waves share no counter and a wave's LDS operations run in order: the result is a function of the ids alone.
 //   one workgroup   (R <= kOneRows): count, scan and place in one launch - a mini-batch costs one launch latency.
 //   three launches  (otherwise): count -> counts[key][chunk]; scan each key's row over the chunks; place.
 // Bound: the ids are read twice and order written once, 2 x 8 + 4 bytes per row with 64-bit ids; the second read of the ids
-// mostly hits the last-level cache.
+// mostly hits the last-level cache.  3.65M rows x 32 groups: 30 us a call (count 6.5, scan 6.6, place 18.9: the 60 vector
+// instructions a slab that find equal keys, and the scattered writes) against 8 us for reading the ids and writing the order once at
+// 5.4 TB/s; up to 8,192 rows 8.5-10 us, the launch and its Python.
 #include "common.hpp"
 
 namespace mcmc {
@@ -20,15 +22,20 @@ constexpr int kOneWaves = 16;           // waves of the one-workgroup kernel
 constexpr int kWaves = 4;               // waves per workgroup of count / place: their four chunks are one int4 of counts
 constexpr int64_t kOneRows = 8192;
 constexpr int kOneKeys = 1024;          // LDS of the one-workgroup kernel: 16 waves x keys x 4 B
-constexpr int kMostChunks = 2048;       // two waves per SIMD
-constexpr int kBatch = 4;               // 64-row slabs whose ids are in flight together
+constexpr int kFewBits = 3;              // up to 8 keys counting by match_key beats 64 LDS additions to few addresses
+constexpr int kMostChunks = 8192;       // eight waves per SIMD (2,048 chunks: 53 us at 3.65M rows x 32 groups, 4,096: 31, 8,192: 30)
+constexpr int kBatch = 4;               // 64-row slabs whose ids are in flight together (2, 4, 8: the same within 1 us)
 
 struct Plan {
     int64_t chunk_rows;  // rows per wave, a multiple of 64
     int chunks;          // a multiple of kWaves
 };
-Plan plan_of(int64_t rows) {
-    int64_t per = (rows + kMostChunks - 1) / kMostChunks;
+// as many chunks as keep the chip busy, but no more counters than half the rows (they are written, scanned and read: at 3.65M rows
+// and 1,000 groups a quarter takes 97 us, half 72, all 77)
+Plan plan_of(int64_t rows, int G) {
+    int64_t most = rows / (2 * ((int64_t)G + 1));
+    most = most < 256 ? 256 : most > kMostChunks ? kMostChunks : most;
+    int64_t per = (rows + most - 1) / most;
     if (per < 512) per = 512;
     per = (per + 63) / 64 * 64;
     int64_t n = (rows + per - 1) / per;
@@ -45,39 +52,53 @@ __device__ __forceinline__ int key_of(const Id* ids, int64_t r, int G) {
 // lanes of the wave with this lane's key (`live` lanes only); bits = bits of the largest key
 __device__ __forceinline__ uint64_t match_key(int key, bool live, int bits) {
     uint64_t m = __ballot(live);
+    uint32_t lo = (uint32_t)m, hi = (uint32_t)(m >> 32);
     for (int b = 0; b < bits; ++b) {
         const uint64_t one = __ballot((key >> b) & 1);
-        m &= ((key >> b) & 1) ? one : ~one;
+        const uint32_t mine = (uint32_t)((key << (31 - b)) >> 31);  // all ones where the bit is set
+        lo &= ~((uint32_t)one ^ mine);
+        hi &= ~((uint32_t)(one >> 32) ^ mine);
     }
-    return m;
+    return (uint64_t)hi << 32 | lo;
 }
 __device__ __forceinline__ int rank_below(uint64_t m, int lane) { return __popcll(m & ((1ull << lane) - 1)); }
 
 // One wave over rows [r0, r1): `run[key]` (LDS, this wave's own) advances by the number of rows of that key; PLACE also writes
-// order[run[key] + rank] = row.  LDS accesses of one wave complete in order, so no barrier is needed between the read of
-// run[] and its update.
+// order[run[key] + rank] = row.  The first lane of each key adds the key's rows of a slab in one LDS operation and hands the old value
+// to the others; a wave's LDS operations complete in order, so the slabs of a batch need no wait between them.
 template <bool PLACE, typename Id>
-__device__ __forceinline__ void walk(const Id* __restrict__ ids, int64_t r0, int64_t r1, int G, int bits, volatile int* run, int* __restrict__ order) {
+__device__ __forceinline__ void walk(const Id* __restrict__ ids, int64_t r0, int64_t r1, int G, int bits, int* run, int* __restrict__ order) {
     const int lane = threadIdx.x & 63;
     for (int64_t base = r0; base < r1; base += 64 * kBatch) {
-        int key[kBatch];
+        int key[kBatch], old[kBatch];
+        uint64_t same[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             const int64_t r = base + 64 * i + lane;
             key[i] = r < r1 ? key_of(ids, r, G) : G;
         }
+        if (!PLACE && bits > kFewBits) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (base + 64 * i + lane < r1) atomicAdd(run + key[i], 1);
+            continue;
+        }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int64_t r = base + 64 * i + lane;
-            const bool live = r < r1;
-            const uint64_t m = match_key(key[i], live, bits);
-            const int rank = rank_below(m, lane);
-            if (live) {
-                const int at = run[key[i]];
-                if (PLACE) order[at + rank] = (int)r;
-                if (rank == 0) run[key[i]] = at + __popcll(m);
+            same[i] = match_key(key[i], base + 64 * i + lane < r1, bits);
+            if (same[i] && rank_below(same[i], lane) == 0 && base + 64 * i + lane < r1) {
+                const int n = __popcll(same[i]);
+                if (PLACE) old[i] = atomicAdd(run + key[i], n);
+                else atomicAdd(run + key[i], n);
             }
         }
+        if (PLACE)
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int64_t r = base + 64 * i + lane;
+                const int at = __shfl(old[i], same[i] ? __ffsll((unsigned long long)same[i]) - 1 : 0);
+                if (r < r1) order[at + rank_below(same[i], lane)] = (int)r;
+            }
     }
 }
 
@@ -211,7 +232,7 @@ int launch(const Id* ids, int64_t rows, int G, int* order, int* offsets, void* w
         group_rows_one_kernel<Id><<<1, 64 * kOneWaves, lds, s>>>(ids, rows, G, bits, order, offsets);
         return check_launch("group_rows_one_kernel");
     }
-    const Plan p = plan_of(rows);
+    const Plan p = plan_of(rows, G);
     const size_t lds = kWaves * (size_t)keys * sizeof(int);
     if (int rc = ensure_dyn_lds((const void*)group_rows_count_kernel<Id>, lds, "group_rows_count_kernel")) return rc;
     if (int rc = ensure_dyn_lds((const void*)group_rows_place_kernel<Id>, lds, "group_rows_place_kernel")) return rc;
@@ -230,7 +251,7 @@ int launch(const Id* ids, int64_t rows, int G, int* order, int* offsets, void* w
 
 int64_t group_rows_workspace_bytes(int64_t rows, int G) {
     if (one_workgroup(rows, G)) return 0;
-    return ((int64_t)(G + 1) * plan_of(rows).chunks + G + 1) * 4;
+    return ((int64_t)(G + 1) * plan_of(rows, G).chunks + G + 1) * 4;
 }
 
 int launch_group_rows(const void* ids, int id_bytes, int64_t rows, int G, int* order, int* offsets, void* ws, hipStream_t s) {
