@@ -164,7 +164,7 @@ constexpr int kThreads = 256;
 //   contraction's end.  Otherwise they pass through registers, element by element where a chunk crosses the end of a row.
 // fp32, one LDS stage (three planes are 48 KB at 128 x 128 x 32: two workgroups a CU, one multiplies while the other stages): the
 // loads of step t+1 are in registers while step t is multiplied, and are split on their way into LDS.
-__device__ const uint4 kZeros = {0, 0, 0, 0};
+__device__ const uint4 kZeros[2] = {};
 constexpr int kSegment = 1024;  // dW: row numbers in LDS, two segments, the next one loaded while one is used
 
 template <int BC>
@@ -215,6 +215,24 @@ __device__ __forceinline__ void store_piece(char* at, int plane_bytes, const Pie
         *reinterpret_cast<bf16x8*>(at + plane_bytes) = m;
         *reinterpret_cast<bf16x8*>(at + 2 * plane_bytes) = l;
     }
+}
+
+// Pieces without a branch between their loads.  whole: every piece has eight elements or none.  Otherwise a piece that ends past its
+// row is read into the next row (`inside` says that there is one) and what is not its own is dropped; a wave with a piece of which
+// that cannot be said reads element by element.
+template <typename T>
+__device__ __forceinline__ Piece<T> load_eight(const T* p, int n) {
+    Piece<T> u;
+    __builtin_memcpy(u.v, n > 0 ? p : reinterpret_cast<const T*>(kZeros), sizeof(u.v));
+    return u;
+}
+template <typename T>
+__device__ __forceinline__ Piece<T> load_through(const T* p, int n, bool inside) {
+    if (__any(n > 0 && n < 8 && !inside)) return load_piece(p, n);
+    Piece<T> u = load_eight(p, n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u.v[i] = i < n ? u.v[i] : (T)0.0f;
+    return u;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -301,7 +319,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     const int steps = (n_c + BC - 1) / BC;
     const T* const P = static_cast<const T*>(a.p);
     const T* const Q = static_cast<const T*>(a.q) + (PRODUCT != kGradWeight && !none ? (int64_t)tl.g * a.n_in * a.n_out : 0);
-    const T* const zeros = reinterpret_cast<const T*>(&kZeros);
+    const T* const zeros = reinterpret_cast<const T*>(kZeros);
 
     // ---- where this lane's pieces come from.  "rows": the chunk's address at step 0, kept.  "columns": row of the tile and first column,
     // made from the lane number where they are used: kept in registers for all pieces they would crowd out the accumulators
@@ -627,21 +645,251 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     }
 }
 
-// dW[g] = the sum of group g's chunks in their order, in 64 bits (free: the kernel waits for memory); the same for db.  One
-// workgroup: 256 elements of one group.
+// ---- short contractions: the weights stay in LDS, the rows stream through registers ------------------------------------------------
+// Forward and dx where the contraction has at most 32 NC elements (a layer of the ensemble's networks, not of wide experts): such a
+// product is bound by reading P and writing the output.  A workgroup takes a run of one group's rows and up to `q_tile` outputs; the
+// weights of those are in LDS as fragments, lane after lane (a fragment is one conflict-free ds_read_b128), and each wave
+// takes 16 rows at a time: their P fragments straight from memory (lane: row l & 15, eight elements from 8 (l >> 4)), no barrier
+// between rows.  The next 16 rows are loaded while these are multiplied, their numbers one step before that.
+// A lane's results are four columns (m = 4 kg .. 4 kg + 3) of each of a 64-column block's four fragments.  fp32: fragment j holds columns
+// 16 j + m.  16-bit: fragments 2 h and 2 h + 1 hold columns 32 h + 8 (m >> 2) + 4 (j & 1) + (m & 3), so that two of them are eight
+// consecutive columns.  Either way a lane stores 16 bytes at a time and the four lanes of a row 64 consecutive bytes.
+constexpr int kStripWaves = 8;
+constexpr int kStripLds = 64 * 1024;  // weights of a workgroup: two workgroups a CU
+
+template <typename T, int PRODUCT, int NC>
+__global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grouped_strip_kernel(Args a, int q_tile, int run_rows) {
+    typedef Frag<T> F;
+    typedef typename F::V V;
+    constexpr int PL = F::kPlanes, NT = 64 * kStripWaves;
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [plane][64-column block][4 j][NC][64 lanes] 16 bytes, then float bias[q_tile]
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, fr = lane & 15, kg = lane >> 4, rows = (int)a.rows;
+    const int n_q = PRODUCT == kForward ? a.n_out : a.n_in, n_c = PRODUCT == kForward ? a.n_in : a.n_out;
+    const int q_tiles = (n_q + q_tile - 1) / q_tile;
+    const int64_t id = xcd_order(blockIdx.x, gridDim.x);  // the q tiles of a run of rows are neighbours
+    const Tile tl = find_tile(a.offsets, a.G, rows, (int)(id / q_tiles), run_rows);
+    if (tl.g < 0) return;
+    const int q0 = (int)(id % q_tiles) * q_tile, width = n_q - q0 < q_tile ? n_q - q0 : q_tile, blocks = (width + 63) / 64;
+    const int plane_bytes = blocks * 4 * NC * 1024;
+    const bool none = tl.g == a.G;
+    const T* const P = static_cast<const T*>(a.p);
+    const T* const W = static_cast<const T*>(a.q) + (none ? 0 : (int64_t)tl.g * a.n_in * a.n_out);
+    float* const bias = reinterpret_cast<float*>(smem + PL * plane_bytes);
+    bool infinite = false;
+
+    // ---- weights and bias -> LDS.  Piece (column, eight contraction elements): consecutive lanes take consecutive columns in dx (W's
+    // rows are read along), consecutive chunks of a column in the forward pass
+    for (int i = t; i < blocks * 64 * NC * 4; i += NT) {
+        const int col = PRODUCT == kForward ? i / (NC * 4) : i % (blocks * 64), ch = PRODUCT == kForward ? i % (NC * 4) : i / (blocks * 64);
+        const int c = 8 * ch, q = q0 + col;
+        const bool have = !none && q < n_q;
+        Piece<T> u;
+        if (PRODUCT == kForward) {
+            u = load_piece(W + (have ? (int64_t)q * a.ld_q + c : 0), have ? n_c - c : 0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u.v[e] = have && c + e < n_c ? W[(int64_t)(c + e) * a.ld_q + q] : (T)0.0f;
+        }
+        const int in = col & 63, j = sizeof(T) == 4 ? in >> 4 : 2 * (in >> 5) + ((in >> 2) & 1);
+        const int m = sizeof(T) == 4 ? in & 15 : 4 * ((in >> 3) & 3) + (in & 3);
+        store_piece(smem + ((((col >> 6) * 4 + j) * NC + (ch >> 2)) * 64 + (ch & 3) * 16 + m) * 16, plane_bytes, u, infinite);
+    }
+    for (int i = t; i < blocks * 64; i += NT)
+        bias[i] = PRODUCT == kForward && a.bias && !none && q0 + i < n_q ? (float)static_cast<const T*>(a.bias)[(int64_t)tl.g * a.n_out + q0 + i] : 0.0f;
+    infinite = __syncthreads_or(infinite);
+
+    auto row_of = [&](int first) { return first + fr < tl.last ? row_at(a, first + fr) : -1; };
+    auto load_rows = [&](int row, Piece<T> (&u)[NC]) {
+        const T* const at = P + (int64_t)(row < 0 ? 0 : row) * a.ld_p + 8 * kg;
+        const int n = row < 0 || none ? 0 : n_c - 8 * kg;
+        if (n_c % 8 == 0) {
+#pragma unroll
+            for (int k = 0; k < NC; ++k) u[k] = load_eight(at + 32 * k, n - 32 * k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < NC; ++k) u[k] = load_through(at + 32 * k, n - 32 * k, row + 1 < rows && 32 * k + 8 * kg + 8 <= a.ld_p + n_c);
+        }
+    };
+    constexpr int kStep = 16 * kStripWaves;
+    int first = tl.first + 16 * wave;
+    int row = row_of(first), row_next = row_of(first + kStep);
+    Piece<T> u[NC];
+    load_rows(row, u);
+    for (; first < tl.last; first += kStep) {
+        V p[PL][NC];
+        bool bad = infinite;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            char piece[PL * 16];
+            store_piece(piece, 16, u[k], bad);
+#pragma unroll
+            for (int l = 0; l < PL; ++l) __builtin_memcpy(&p[l][k], piece + 16 * l, 16);
+        }
+        const int out_row = row;
+        row = row_next;
+        if (first + kStep < tl.last) {
+            load_rows(row, u);
+            row_next = row_of(first + 2 * kStep);
+        }
+        T* const out = static_cast<T*>(a.out) + (int64_t)(out_row < 0 ? 0 : out_row) * n_q + q0;
+        auto column = [&](int b, int j) { return 64 * b + (sizeof(T) == 4 ? 16 * j + 4 * kg : 32 * (j >> 1) + 8 * kg + 4 * (j & 1)); };
+        for (int b = 0; b < blocks; ++b) {
+            f32x4 acc[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = *reinterpret_cast<const f32x4*>(bias + column(b, j));
+            const char* w = smem + (b * 4 * NC * 64 + lane) * 16;
+#pragma unroll
+            for (int l = PL - 1; l >= 0; --l)  // small products first, as in the tile kernel
+#pragma unroll
+                for (int m = PL - 1 - l; m >= 0; --m)
+#pragma unroll
+                    for (int k = 0; k < NC; ++k)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            acc[j] = F::mfma(*reinterpret_cast<const V*>(w + m * plane_bytes + (j * NC + k) * 1024), p[l][k], acc[j]);
+            if (sizeof(T) == 4 && __any(bad)) {  // an infinity: element by element (see Frag<float>)
+                for (int j = 0; j < 4; ++j)
+                    for (int e = 0; e < 4; ++e) {
+                        const int q = q0 + column(b, j) + e;
+                        float v = bias[q - q0];
+                        if (out_row >= 0 && q < n_q && !none)
+                            for (int c = 0; c < n_c; ++c)
+                                v = fmaf((float)P[(int64_t)out_row * a.ld_p + c], (float)W[PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)c * a.ld_q + q], v);
+                        acc[j][e] = v;
+                    }
+            }
+            if (out_row < 0) continue;
+            constexpr int kOnce = 16 / sizeof(T);  // columns a store takes
+            typedef T Some __attribute__((ext_vector_type(kOnce)));
+            typedef Some Anywhere __attribute__((aligned(sizeof(T))));
+#pragma unroll
+            for (int h = 0; h < 16 / kOnce; ++h) {
+                const int q = column(b, h * (kOnce / 4));
+                Some o;
+#pragma unroll
+                for (int e = 0; e < kOnce; ++e) o[e] = (T)acc[h * (kOnce / 4) + (e >> 2)][e & 3];
+                if (q + kOnce <= width) {
+                    *reinterpret_cast<Anywhere*>(out + q) = o;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kOnce; ++e)
+                        if (q + e < width) out[q + e] = o[e];
+                }
+            }
+        }
+    }
+}
+
+// ---- dW where one side is a handful of columns (the output layer, the first layer) ------------------------------------------------
+// dW[t][c] = sum_r thin[r][t] wide[r][c], at most 16 columns t: bound by reading the wide rows once.  On the fp32 matrix
+// instructions (16 x 16 outputs, 4 rows each), whose operands need no turning: lane (fr, kg) holds thin[row kg][fr] and, for instruction
+// j, wide[row kg][8 fr + j] - it loads its 8 columns of a row in one access and 16 lanes load a row's 128 side by side.  Exact for
+// 16-bit operands, plain fp32 sums for fp32.  Four waves take turns at 64 rows of a run and meet in LDS in their order.
+// THIN_OUT: thin = dy (n_out columns), db is its column sum; otherwise thin = x (n_in <= 15), and db comes from a column of ones.
+constexpr int kThinMost = 16;
+constexpr int kThinCols = 128;
+
+template <typename T, bool THIN_OUT>
+__global__ __launch_bounds__(256) void grouped_thin_kernel(Args a) {
+    __shared__ float sums[4][kThinMost][kThinCols];
+    __shared__ float sums_b[4][kThinMost];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, fr = lane & 15, kg = lane >> 4, rows = (int)a.rows;
+    const T* const thin = static_cast<const T*>(THIN_OUT ? a.p : a.q);
+    const T* const wide = static_cast<const T*>(THIN_OUT ? a.q : a.p);
+    const int64_t ld_t = THIN_OUT ? a.ld_p : a.ld_q, ld_w = THIN_OUT ? a.ld_q : a.ld_p;
+    const int n_t = THIN_OUT ? a.n_out : a.n_in, n_w = THIN_OUT ? a.n_in : a.n_out;
+    const int col_blocks = (n_w + kThinCols - 1) / kThinCols, run = blockIdx.x / col_blocks, w0 = blockIdx.x % col_blocks * kThinCols;
+    Tile tl;
+    if (a.chunk_rows) {
+        tl = find_tile(a.offsets, a.G, rows, run, a.chunk_rows);
+        if (tl.g < 0 || tl.g >= a.G || run >= a.chunks) return;
+    } else {
+        tl.g = run;
+        runs_of(a.offsets, a.G, rows, run, 1, tl.first, tl.last);
+    }
+    const int c = w0 + 8 * fr;
+    f32x4 acc[8] = {};
+    float sum_b = 0.0f;
+    for (int first = tl.first + 64 * wave; first < tl.last; first += 256) {
+        const int mine = first + lane < tl.last ? row_at(a, first + lane) : -1;
+#pragma unroll 1
+        for (int s0 = 0; s0 < 16; s0 += 4) {
+            Piece<T> w[4];
+            T th[4];
+            int row[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                row[s] = __shfl(mine, 4 * (s0 + s) + kg);
+                th[s] = *(row[s] >= 0 && fr < n_t ? thin + (int64_t)row[s] * ld_t + fr : reinterpret_cast<const T*>(kZeros));
+            }
+            if (n_w % 8 == 0) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) w[s] = load_eight(wide + (int64_t)row[s] * ld_w + c, row[s] < 0 ? 0 : n_w - c);
+            } else {
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    w[s] = load_through(wide + (int64_t)row[s] * ld_w + c, row[s] < 0 ? 0 : n_w - c, row[s] + 1 < rows && c + 8 <= ld_w + n_w);
+            }
+            if (!THIN_OUT && fr == n_t)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) th[s] = row[s] >= 0 ? (T)1.0f : (T)0.0f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                if (THIN_OUT) sum_b += (float)th[s];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)th[s], (float)w[s].v[j], acc[j], 0, 0, 0);
+            }
+        }
+    }
+    // lane: thin columns 4 kg + i, wide columns 8 fr + j
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[wave][4 * kg + i][8 * fr + j] = acc[j][i];
+    sum_b += __shfl_xor(sum_b, 16);
+    sum_b += __shfl_xor(sum_b, 32);
+    if (kg == 0) sums_b[wave][fr] = sum_b;
+    __syncthreads();
+    const int64_t n = (int64_t)a.n_out * a.n_in, at = (int64_t)run * n, at_b = (a.chunk_rows ? (int64_t)a.chunks * n : 0) + (int64_t)run * a.n_out;
+    auto put = [&](bool b, int64_t i, float v) {
+        if (a.chunk_rows) a.part[i] = v;
+        else static_cast<T*>(b ? a.dbias : a.out)[i] = (T)v;
+    };
+    for (int i = t; i < kThinMost * kThinCols; i += 256) {
+        const int th = THIN_OUT ? i / kThinCols : i % kThinMost, w = THIN_OUT ? i % kThinCols : i / kThinMost;
+        if (w0 + w >= n_w) continue;
+        const float v = sums[0][th][w] + sums[1][th][w] + sums[2][th][w] + sums[3][th][w];
+        if (th < n_t) put(false, at + (THIN_OUT ? (int64_t)th * a.n_in + w0 + w : (int64_t)(w0 + w) * a.n_in + th), v);
+        else if (!THIN_OUT && a.dbias && th == n_t) put(true, at_b + w0 + w, v);
+    }
+    if (THIN_OUT && a.dbias && w0 == 0 && t < n_t) put(true, at_b + t, sums_b[0][t] + sums_b[1][t] + sums_b[2][t] + sums_b[3][t]);
+}
+
+// dW[g] = the sum of group g's chunks, in 64 bits (free: the kernel waits for memory); the same for db.  A workgroup sums 32 elements of
+// one group: eight slices of the chunks, each in its order, then the slices in theirs.
+constexpr int kSumElems = 32;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void grouped_sum_kernel(Args a) {
+    __shared__ double part[kThreads / kSumElems][kSumElems];
     const int64_t n = (int64_t)a.n_out * a.n_in, all = n + (a.dbias ? a.n_out : 0);
-    const int64_t blocks = (all + kThreads - 1) / kThreads;
-    const int g = (int)(blockIdx.x / blocks);
-    const int first = runs_before(a.offsets, a.G, g, (int)a.rows, a.chunk_rows), end = runs_before(a.offsets, a.G, g + 1, (int)a.rows, a.chunk_rows);
+    const int64_t blocks = (all + kSumElems - 1) / kSumElems;
+    const int g = (int)(blockIdx.x / blocks), e = threadIdx.x % kSumElems, slice = threadIdx.x / kSumElems;
+    const int first = runs_before(a.offsets, a.G, g, (int)a.rows, a.chunk_rows);
+    int b, end;
+    end = first + runs_of(a.offsets, a.G, (int)a.rows, g, a.chunk_rows, b, end);
     const int last = end < a.chunks ? end : a.chunks;
-    const int64_t i = (int64_t)(blockIdx.x % blocks) * kThreads + threadIdx.x;
-    if (i >= all) return;
-    const float* src = i < n ? a.part + i : a.part + (int64_t)a.chunks * n + (i - n);
-    const int64_t step = i < n ? n : a.n_out;
+    const int64_t i = (int64_t)(blockIdx.x % blocks) * kSumElems + e;
     double s = 0.0;
-    for (int c = first; c < last; ++c) s += (double)src[c * step];
+    if (i < all) {
+        const float* src = i < n ? a.part + i : a.part + (int64_t)a.chunks * n + (i - n);
+        const int64_t step = i < n ? n : a.n_out;
+#pragma unroll 4
+        for (int c = first + slice; c < last; c += kThreads / kSumElems) s += (double)src[c * step];
+    }
+    part[slice][e] = s;
+    __syncthreads();
+    if (slice != 0 || i >= all) return;
+    for (int k = 1; k < kThreads / kSumElems; ++k) s += part[k][e];
     if (i < n) static_cast<T*>(a.out)[g * n + i] = (T)s;
     else static_cast<T*>(a.dbias)[(int64_t)g * a.n_out + (i - n)] = (T)s;
 }
@@ -698,9 +946,48 @@ int launch_product(const Args& a, Shape sh, bool dma, unsigned blocks, hipStream
     }
 }
 
+// The strip kernel for contractions of up to 256 elements (fp32: 128) whose weights fit two workgroups' LDS: all of them, or, where
+// the contraction is so short (64) that reading P again for every q_tile columns costs little beside the output, any number.
+// Returns 0 where the tile kernel is to run.
+template <typename T>
+int strip_q_tile(int n_c, int n_q) {
+    const int steps = ceil_div(n_c, 32), nc = steps <= 1 ? 1 : steps <= 2 ? 2 : steps <= 4 ? 4 : 8;
+    const int tile = kStripLds / (nc * 64 * Frag<T>::kPlanes) / 64 * 64;
+    if (steps > 8 || tile == 0 || (n_q > tile && nc > 2)) return 0;
+    return ceil_div(n_q, 64) * 64 < tile ? ceil_div(n_q, 64) * 64 : tile;
+}
+
+template <typename T, int PRODUCT, int NC>
+int launch_strip_n(const Args& a, int q_tile, int run, unsigned blocks, hipStream_t s) {
+    const size_t lds = (size_t)NC * 64 * Frag<T>::kPlanes * q_tile + q_tile * sizeof(float);
+    const auto kern = grouped_strip_kernel<T, PRODUCT, NC>;
+    if (int rc = ensure_dyn_lds((const void*)kern, lds, "grouped_strip_kernel")) return rc;
+    kern<<<blocks, 64 * kStripWaves, lds, s>>>(a, q_tile, run);
+    return check_launch("grouped_strip_kernel");
+}
+
+template <typename T, int PRODUCT>
+int launch_strip(const Args& a, int q_tile, hipStream_t s) {
+    const int n_q = PRODUCT == kForward ? a.n_out : a.n_in, n_c = PRODUCT == kForward ? a.n_in : a.n_out;
+    // rows per workgroup: about two workgroups a CU and round, whole turns of its waves, weights loaded once for many rows
+    int64_t run = a.rows / 1024 / (16 * kStripWaves) * (16 * kStripWaves);
+    run = run < 16 * kStripWaves ? 16 * kStripWaves : run > 4096 ? 4096 : run;
+    const int64_t blocks = (a.rows / run + (a.G + 1 < a.rows ? a.G + 1 : a.rows)) * ceil_div(n_q, q_tile);
+    if (int rc = check_grid(blocks)) return rc;
+    if (n_c <= 32) return launch_strip_n<T, PRODUCT, 1>(a, q_tile, (int)run, (unsigned)blocks, s);
+    if (n_c <= 64) return launch_strip_n<T, PRODUCT, 2>(a, q_tile, (int)run, (unsigned)blocks, s);
+    if (n_c <= 128) return launch_strip_n<T, PRODUCT, 4>(a, q_tile, (int)run, (unsigned)blocks, s);
+    if constexpr (sizeof(T) == 2) return launch_strip_n<T, PRODUCT, 8>(a, q_tile, (int)run, (unsigned)blocks, s);
+    return MCMC_EINVAL;  // strip_q_tile takes no fp32 contraction beyond 128
+}
+
 template <typename T>
 int launch(int product, const Args& a, hipStream_t s) {
     const int n_q = product == kForward ? a.n_out : a.n_in;
+    if (product != kGradWeight) {
+        if (const int q_tile = strip_q_tile<T>(product == kForward ? a.n_in : a.n_out, n_q))
+            return product == kForward ? launch_strip<T, kForward>(a, q_tile, s) : launch_strip<T, kGradInput>(a, q_tile, s);
+    }
     const bool dma = sizeof(T) == 2 && whole_chunks(product, a);
     const Shape sh = shape_of(product, dma, a.rows, a.G, a.n_in, a.n_out);
     const int64_t runs = product == kGradWeight ? (int64_t)ceil_div(a.n_out, sh.bp) * (a.chunk_rows ? a.chunks : a.G)
@@ -709,9 +996,18 @@ int launch(int product, const Args& a, hipStream_t s) {
     if (int rc = check_grid(blocks)) return rc;
     if (product == kForward) return launch_product<T, kForward>(a, sh, dma, (unsigned)blocks, s);
     if (product == kGradInput) return launch_product<T, kGradInput>(a, sh, dma, (unsigned)blocks, s);
-    if (int rc = launch_product<T, kGradWeight>(a, sh, dma, (unsigned)blocks, s)) return rc;
+    const bool thin_out = a.n_out <= kThinMost;
+    if (thin_out || a.n_in < kThinMost) {
+        const int64_t thin = (int64_t)ceil_div(thin_out ? a.n_in : a.n_out, kThinCols) * (a.chunk_rows ? a.chunks : a.G);
+        if (int rc = check_grid(thin)) return rc;
+        if (thin_out) grouped_thin_kernel<T, true><<<(unsigned)thin, 256, 0, s>>>(a);
+        else grouped_thin_kernel<T, false><<<(unsigned)thin, 256, 0, s>>>(a);
+        if (int rc = check_launch("grouped_thin_kernel")) return rc;
+    } else if (int rc = launch_product<T, kGradWeight>(a, sh, dma, (unsigned)blocks, s)) {
+        return rc;
+    }
     if (!a.chunk_rows) return MCMC_OK;
-    const int64_t sums = ((int64_t)a.n_out * a.n_in + (a.dbias ? a.n_out : 0) + kThreads - 1) / kThreads * a.G;
+    const int64_t sums = ((int64_t)a.n_out * a.n_in + (a.dbias ? a.n_out : 0) + kSumElems - 1) / kSumElems * a.G;
     if (int rc = check_grid(sums)) return rc;
     grouped_sum_kernel<T><<<(unsigned)sums, kThreads, 0, s>>>(a);
     return check_launch("grouped_sum_kernel");
