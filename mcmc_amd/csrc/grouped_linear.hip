@@ -124,23 +124,41 @@ __device__ __forceinline__ int runs_before(const int* __restrict__ offsets, int 
     for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
     return n;
 }
-// The `tile`-th run of at most `per` rows, group after group (each group starts a run of its own), then the rows of no group.
-// A wave looks at 64 groups at a time: their run counts, a prefix sum over the lanes, the lane whose group holds the tile.
-__device__ __forceinline__ Tile find_tile(const int* __restrict__ offsets, int G, int rows, int tile, int per) {
+// The runs of at most `per` rows, group after group (each group starts runs of its own), then those of the rows of no group.  A wave looks
+// at 64 groups at a time: their run counts, a prefix sum over the lanes.  Up to 63 groups are looked at once for both questions.
+struct Runs {
+    int total;                         // runs of groups 0 .. last_group
+    int first, last, count, inclusive; // this lane's group, if one look is enough
+};
+__device__ __forceinline__ Runs count_runs(const int* __restrict__ offsets, int G, int rows, int per, int last_group) {
+    Runs r;
+    r.count = runs_of(offsets, G, rows, threadIdx.x & 63, per, r.first, r.last);
+    if ((threadIdx.x & 63) > last_group) r.count = 0;
+    r.inclusive = wave_inclusive(r.count);
+    r.total = G < 64 ? __shfl(r.inclusive, 63) : runs_before(offsets, G, last_group + 1, rows, per);
+    return r;
+}
+__device__ __forceinline__ Tile nth_run(const int* __restrict__ offsets, int G, int rows, int per, const Runs& r, int n) {
     int before = 0;
     for (int g0 = 0; g0 <= G; g0 += 64) {
-        int b, e;
-        const int n = runs_of(offsets, G, rows, g0 + (threadIdx.x & 63), per, b, e), inc = wave_inclusive(n);
-        const uint64_t hit = __ballot(before + inc > tile);
+        int b = r.first, e = r.last, count = r.count, inc = r.inclusive;
+        if (g0 > 0 || G >= 64) {
+            count = runs_of(offsets, G, rows, g0 + (threadIdx.x & 63), per, b, e);
+            inc = wave_inclusive(count);
+        }
+        const uint64_t hit = __ballot(before + inc > n);
         if (hit) {
             const int l = __ffsll((unsigned long long)hit) - 1;
-            const int start = __shfl(b, l), end = __shfl(e, l), mine = tile - before - (__shfl(inc, l) - __shfl(n, l));
+            const int start = __shfl(b, l), end = __shfl(e, l), mine = n - before - (__shfl(inc, l) - __shfl(count, l));
             const int64_t first = (int64_t)start + (int64_t)mine * per;
             return Tile{g0 + l, (int)first, (int)(first + per < end ? first + per : end)};
         }
         before += __shfl(inc, 63);
     }
     return Tile{-1, 0, 0};
+}
+__device__ __forceinline__ Tile find_tile(const int* __restrict__ offsets, int G, int rows, int n, int per) {
+    return nth_run(offsets, G, rows, per, count_runs(offsets, G, rows, per, G), n);
 }
 
 __device__ __forceinline__ int row_at(const Args& a, int pos) {
@@ -286,9 +304,10 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     if (PRODUCT == kGradWeight) {
         const int p_tiles = (a.n_out + BP - 1) / BP, per_run = p_tiles * q_tiles;
         int64_t runs = a.G;
+        Runs all;
         if (a.chunk_rows) {
-            runs = runs_before(a.offsets, a.G, a.G, rows, a.chunk_rows);
-            runs = runs < a.chunks ? runs : a.chunks;  // (offsets that decrease could ask for more)
+            all = count_runs(a.offsets, a.G, rows, a.chunk_rows, a.G - 1);
+            runs = all.total < a.chunks ? all.total : a.chunks;  // (offsets that decrease could ask for more)
         }
         if ((int64_t)blockIdx.x >= runs * per_run) return;
         id = xcd_order(blockIdx.x, runs * per_run);
@@ -298,18 +317,19 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         p0 = (band * kBand + at % high) * BP;
         q0 = at / high * BQ;
         if (a.chunk_rows) {
-            tl = find_tile(a.offsets, a.G, rows, run, a.chunk_rows);
+            tl = nth_run(a.offsets, a.G, rows, a.chunk_rows, all, run);
         } else {
             tl.g = run;
             runs_of(a.offsets, a.G, rows, run, 1, tl.first, tl.last);
         }
     } else {
-        const int64_t tiles = runs_before(a.offsets, a.G, a.G + 1, rows, BP);
+        const Runs all = count_runs(a.offsets, a.G, rows, BP, a.G);
+        const int64_t tiles = all.total;
         if ((int64_t)blockIdx.x >= tiles * q_tiles) return;
         id = xcd_order(blockIdx.x, tiles * q_tiles);
         const int64_t band = id / (kBand * q_tiles), left = tiles - band * kBand, high = left < kBand ? left : kBand;
         const int64_t at = id - band * kBand * q_tiles;
-        tl = find_tile(a.offsets, a.G, rows, (int)(band * kBand + at % high), BP);
+        tl = nth_run(a.offsets, a.G, rows, BP, all, (int)(band * kBand + at % high));
         q0 = (int)(at / high) * BQ;
         for (int i = t; i < BP; i += NT) rows_lds[i] = tl.first + i < tl.last ? row_at(a, tl.first + i) : -1;
         __syncthreads();
@@ -622,9 +642,13 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             const int q = q0 + qw + 16 * j + 4 * kg;
             const f32x4 v = acc[i][j];
             if (PRODUCT == kGradWeight && a.chunk_rows) {
+                if (n_q % 4 == 0) {
+                    if (q < n_q) *reinterpret_cast<f32x4*>(a.part + at + q) = v;
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (q + e < n_q) a.part[at + q + e] = v[e];
+                    for (int e = 0; e < 4; ++e)
+                        if (q + e < n_q) a.part[at + q + e] = v[e];
+                }
             } else if (whole) {
                 typedef T T4 __attribute__((ext_vector_type(4)));
                 if (q < n_q) *reinterpret_cast<T4*>(static_cast<T*>(a.out) + at + q) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
@@ -865,31 +889,34 @@ __global__ __launch_bounds__(256) void grouped_thin_kernel(Args a) {
     if (THIN_OUT && a.dbias && w0 == 0 && t < n_t) put(true, at_b + t, sums_b[0][t] + sums_b[1][t] + sums_b[2][t] + sums_b[3][t]);
 }
 
-// dW[g] = the sum of group g's chunks, in 64 bits (free: the kernel waits for memory); the same for db.  A workgroup sums 32 elements of
-// one group: eight slices of the chunks, each in its order, then the slices in theirs.
-constexpr int kSumElems = 32;
-template <typename T>
+// dW[g] = the sum of group g's chunks, in 64 bits (free: the kernel waits for memory); the same for db.  A workgroup sums 256 / SLICES
+// elements of one group: each slice of the chunks in its order, then the slices in theirs.
+template <typename T, int SLICES>
 __global__ __launch_bounds__(kThreads) void grouped_sum_kernel(Args a) {
-    __shared__ double part[kThreads / kSumElems][kSumElems];
+    constexpr int kElems = kThreads / SLICES;
+    __shared__ double part[SLICES][kElems];
     const int64_t n = (int64_t)a.n_out * a.n_in, all = n + (a.dbias ? a.n_out : 0);
-    const int64_t blocks = (all + kSumElems - 1) / kSumElems;
-    const int g = (int)(blockIdx.x / blocks), e = threadIdx.x % kSumElems, slice = threadIdx.x / kSumElems;
+    const int64_t blocks = (all + kElems - 1) / kElems;
+    const int g = (int)(blockIdx.x / blocks), e = threadIdx.x % kElems, slice = threadIdx.x / kElems;
     const int first = runs_before(a.offsets, a.G, g, (int)a.rows, a.chunk_rows);
     int b, end;
     end = first + runs_of(a.offsets, a.G, (int)a.rows, g, a.chunk_rows, b, end);
     const int last = end < a.chunks ? end : a.chunks;
-    const int64_t i = (int64_t)(blockIdx.x % blocks) * kSumElems + e;
+    const int64_t i = (int64_t)(blockIdx.x % blocks) * kElems + e;
     double s = 0.0;
     if (i < all) {
         const float* src = i < n ? a.part + i : a.part + (int64_t)a.chunks * n + (i - n);
         const int64_t step = i < n ? n : a.n_out;
-#pragma unroll 4
-        for (int c = first + slice; c < last; c += kThreads / kSumElems) s += (double)src[c * step];
+#pragma unroll 8
+        for (int c = first + slice; c < last; c += SLICES) s += (double)src[c * step];
     }
-    part[slice][e] = s;
-    __syncthreads();
-    if (slice != 0 || i >= all) return;
-    for (int k = 1; k < kThreads / kSumElems; ++k) s += part[k][e];
+    if (SLICES > 1) {
+        part[slice][e] = s;
+        __syncthreads();
+        if (slice != 0) return;
+        for (int k = 1; k < SLICES; ++k) s += part[k][e];
+    }
+    if (i >= all) return;
     if (i < n) static_cast<T*>(a.out)[g * n + i] = (T)s;
     else static_cast<T*>(a.dbias)[(int64_t)g * a.n_out + (i - n)] = (T)s;
 }
@@ -909,7 +936,7 @@ Shape shape_of(int product, bool dma, int64_t rows, int G, int n_in, int n_out) 
 int chunk_rows_of(int64_t rows, int G, int n_in, int n_out) {
     const int64_t tiles = (int64_t)ceil_div(n_out, 128) * ceil_div(n_in, 128);
     if (tiles * G >= 512 || rows <= 512) return 0;
-    int64_t per = ceil_div(rows * tiles, 1024);
+    int64_t per = ceil_div(rows * tiles, tiles <= 4 ? 1024 : 512);  // (the larger dW is, the more its partial sums cost)
     per = (per + 255) / 256 * 256;
     return per >= rows ? 0 : (int)per;
 }
@@ -1007,9 +1034,12 @@ int launch(int product, const Args& a, hipStream_t s) {
         return rc;
     }
     if (!a.chunk_rows) return MCMC_OK;
-    const int64_t sums = ((int64_t)a.n_out * a.n_in + (a.dbias ? a.n_out : 0) + kSumElems - 1) / kSumElems * a.G;
+    // few chunks a group: a thread sums them all; many: eight threads share them
+    const int slices = a.chunks / a.G > 16 ? 8 : 1;
+    const int64_t sums = ((int64_t)a.n_out * a.n_in + (a.dbias ? a.n_out : 0) + kThreads / slices - 1) / (kThreads / slices) * a.G;
     if (int rc = check_grid(sums)) return rc;
-    grouped_sum_kernel<T><<<(unsigned)sums, kThreads, 0, s>>>(a);
+    if (slices == 8) grouped_sum_kernel<T, 8><<<(unsigned)sums, kThreads, 0, s>>>(a);
+    else grouped_sum_kernel<T, 1><<<(unsigned)sums, kThreads, 0, s>>>(a);
     return check_launch("grouped_sum_kernel");
 }
 
