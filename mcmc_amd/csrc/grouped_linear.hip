@@ -176,6 +176,9 @@ constexpr int kThreads = 256;
 //   "columns" [BC][BP or BQ]     operands whose output index is contiguous (W in dx; both in dW); fragments by ds_read_b64_tr_b16,
 //             which hands each lane a column of four rows.  The 32-byte chunks of row c are permuted by spread(c): the eight rows a
 //             pass touches ({0-3, 8-11} + 4n) hit all banks.
+// A fragment's 16 rows or columns follow each other in the tile, but for Q's of 16-bit types ("paired"): fragments 2 h and 2 h + 1 hold
+// 32 h + 8 (m >> 2) + 4 (j & 1) + (m & 3), so that a lane's results of two fragments are eight consecutive columns, one 16-byte
+// store, and the four lanes of an output row store 64 consecutive bytes.
 // 16-bit types, two LDS stages: the loads of step t+1 run while step t is multiplied, one barrier a step.
 //   DMA: every row starts on 16 bytes and holds whole 8-element chunks: the pieces go global -> LDS directly (the permutation is
 //   on the global side, a wave-instruction fills 1 KiB of LDS in order), 16 zero bytes stand in for what lies past the
@@ -185,9 +188,12 @@ constexpr int kThreads = 256;
 __device__ const uint4 kZeros[2] = {};
 constexpr int kSegment = 1024;  // dW: row numbers in LDS, two segments, the next one loaded while one is used
 
-template <int BC>
-__device__ __forceinline__ int turn(int r) {  // permutation of the 16-byte pieces of row r
-    return BC == 64 ? r & 7 : -(r >> 2) & 3;
+// permutation of the 16-byte pieces of row r: a pass of ds_read_b128 takes fragment rows {0-3, 12-15} of one lane group and {4-11} of the
+// next; PAIRED: row m of the fragment is row 8 (m >> 2) + (m & 3) of the tile
+template <int BC, bool PAIRED>
+__device__ __forceinline__ int turn(int r) {
+    if (BC == 64) return PAIRED ? (r & 3) | ((r >> 1) & 4) : r & 7;
+    return -(r >> (PAIRED ? 3 : 2)) & 3;
 }
 template <int B>
 __device__ __forceinline__ int spread(int c) {  // bytes to xor: bits 5.. of the offset in row c
@@ -270,6 +276,23 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// row[q .. q + N - 1] = value(0 .. N - 1) as far as the row goes: one store of 16 bytes, which may lie anywhere, or element by element
+template <typename T, int N, typename Value>
+__device__ __forceinline__ void store_some(T* row, int q, int width, Value value) {
+    typedef T Some __attribute__((ext_vector_type(N)));
+    typedef Some Anywhere __attribute__((aligned(sizeof(T))));
+    Some o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = (T)value(e);  // the one rounding of a 16-bit result
+    if (q + N <= width) {
+        *reinterpret_cast<Anywhere*>(row + q) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (q + e < width) row[q + e] = o[e];
+    }
+}
+
 // workgroup id -> tile id: ids go round the eight XCDs, each XCD gets a contiguous run of tiles (its L2 sees neighbours)
 __device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t n) {
     const int64_t x = id & 7, i = id >> 3, q = n >> 3, r = n & 7;
@@ -282,6 +305,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     typedef typename F::V V;
     constexpr bool kWide = sizeof(T) == 4;
     constexpr int NW = WP * WQ, NT = 64 * NW;
+    constexpr bool kPair = !kWide;
     constexpr bool kAhead = STAGES == 1;  // one stage: the next step waits in registers
     static_assert(DMA ? STAGES >= 2 : STAGES <= 2, "");
     constexpr bool kPCols = PRODUCT == kGradWeight, kQCols = PRODUCT != kForward;
@@ -345,14 +369,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     // made from the lane number where they are used: kept in registers for all pieces they would crowd out the accumulators
     // (`now_lane` is the lane number behind an empty asm statement, so that the compiler does not move the arithmetic out of the loop).
     const T *src_p[kPCols ? 1 : NP], *src_q[kQCols ? 1 : NQ];
-    int c_p = 0, c_q = 0;  // "rows": first element of the chunk at step 0 (every piece of a lane has the same one)
+    int c_p = 0, c_q[kQCols ? 1 : NQ];  // "rows": first element of the chunk at step 0 (all of P's pieces of a lane have the same one)
     int now_lane = lane;
     auto col_row = [&](int n, int np, int b) { return ((wave * np + n) * 64 + now_lane) / (b / 8); };
     if constexpr (!kPCols) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const int piece = (wave * NP + n) * 64 + lane, r = piece / (BC / 8), row = rows_lds[r] < 0 ? 0 : rows_lds[r];
-            c_p = 8 * ((piece % (BC / 8)) ^ turn<BC>(r));
+            c_p = 8 * ((piece % (BC / 8)) ^ turn<BC, false>(r));
             src_p[n] = P + (int64_t)row * a.ld_p + c_p;  // rows past the end: any, not stored
         }
     }
@@ -360,8 +384,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             const int piece = (wave * NQ + n) * 64 + lane, r = piece / (BC / 8), row = q0 + r < n_q ? q0 + r : n_q - 1;
-            c_q = 8 * ((piece % (BC / 8)) ^ turn<BC>(r));
-            src_q[n] = Q + (int64_t)row * a.ld_q + c_q;
+            c_q[n] = 8 * ((piece % (BC / 8)) ^ turn<BC, kPair>(r));
+            src_q[n] = Q + (int64_t)row * a.ld_q + c_q[n];
         }
     }
     // dW: row numbers of the run's positions 1024 s .. 1024 s + 1023 -> LDS
@@ -422,7 +446,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
                 if (DMA && col >= n_q) col = 0;
                 p = Q + (int64_t)r * a.ld_q + col;
             } else {
-                have = n_c - c0 - c_q;
+                have = n_c - c0 - c_q[m];
                 p = src_q[m] + c0;
             }
             to += kPBytes * F::kPlanes + (wave * NQ + m) * 1024;
@@ -446,34 +470,43 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 
     // ---- fragments
     const int pw = BP / WP * (wave % WP), qw = BQ / WQ * (wave / WP), fr = lane & 15, kg = lane >> 4;
-    // byte offset of fragment 0 in its tile; fragment i: "rows" + 16 i rows, "columns" ^ 32 i (no carry: 16 x fragments divides a
-    // wave's first column).  The second 32 contraction elements: "rows" ^ 64, "columns" + 32 rows.
-    auto frag_at = [&](auto cols, auto width, int first) {
+    // byte offset of fragment 0 in its tile; fragment i: "rows" + 16 i rows, "columns" ^ 32 i; paired "rows" + 32 (i >> 1) + 4 (i & 1)
+    // rows, "columns" ^ 64 (i >> 1) + 8 (i & 1) (no carry: a wave's first column is a multiple of all its fragments' columns).  The
+    // second 32 contraction elements: "rows" ^ 64, "columns" + 32 rows.
+    auto frag_at = [&](auto cols, auto paired, auto width, int first) {
         constexpr int B = decltype(width)::value;
+        constexpr bool kTwo = decltype(paired)::value;
         if constexpr (decltype(cols)::value) {
             const int c = 8 * kg + (fr >> 2);  // rows c and c + 4
-            return c * (2 * B) + ((2 * first) ^ spread<B>(c)) + 8 * (fr & 3);
+            return c * (2 * B) + ((2 * first + (kTwo ? 16 * (fr & 3) : 0)) ^ spread<B>(c)) + (kTwo ? 0 : 8 * (fr & 3));
         } else {
-            return (first + fr) * (2 * BC) + ((kg ^ turn<BC>(fr)) << 4);
+            const int r = kTwo ? 8 * (fr >> 2) + (fr & 3) : fr;
+            return (first + r) * (2 * BC) + ((kg ^ turn<BC, kTwo>(r)) << 4);
         }
     };
-    auto frag = [&](auto cols, auto width, const char* tile, int at, int i, int kk) -> V {
+    auto frag = [&](auto cols, auto paired, auto width, const char* tile, int at, int i, int kk) -> V {
         constexpr int B = decltype(width)::value;
-        if constexpr (decltype(cols)::value) return columns_frag<V>(tile + (at ^ (32 * i)) + kk * 32 * (2 * B), 4 * 2 * B);
-        else return *reinterpret_cast<const V*>(tile + (at ^ (64 * kk)) + 16 * i * (2 * BC));
+        constexpr bool kTwo = decltype(paired)::value;
+        if constexpr (decltype(cols)::value)
+            return columns_frag<V>(tile + (at ^ (kTwo ? 64 * (i >> 1) : 32 * i)) + (kTwo ? 8 * (i & 1) : 0) + kk * 32 * (2 * B), 4 * 2 * B);
+        else
+            return *reinterpret_cast<const V*>(tile + (at ^ (64 * kk)) + (kTwo ? 32 * (i >> 1) + 4 * (i & 1) : 16 * i) * (2 * BC));
     };
-    int at_p = frag_at(std::integral_constant<bool, kPCols>(), std::integral_constant<int, BP>(), pw);
-    int at_q = frag_at(std::integral_constant<bool, kQCols>(), std::integral_constant<int, BQ>(), qw);
+    typedef std::integral_constant<bool, kPCols> PCols;
+    typedef std::integral_constant<bool, kQCols> QCols;
+    typedef std::integral_constant<bool, kPair> Pair;
+    int at_p = frag_at(PCols(), std::false_type(), std::integral_constant<int, BP>(), pw);
+    int at_q = frag_at(QCols(), Pair(), std::integral_constant<int, BQ>(), qw);
     f32x4 acc[FP][FQ] = {};
     // db: this lane's share of the sums of dy's columns.  fp32 results: a plain sum loses more than torch's pairwise one, so every
     // kSegment rows the running sum goes into a second one
     float accb[FP] = {}, sumb[FP] = {};
     const bool sum_bias = PRODUCT == kGradWeight && a.dbias && q0 == 0 && qw == 0;
     auto p_frag = [&](const char* stage, int l, int i, int kk) {
-        return frag(std::integral_constant<bool, kPCols>(), std::integral_constant<int, BP>(), stage + l * kPBytes, at_p, i, kk);
+        return frag(PCols(), std::false_type(), std::integral_constant<int, BP>(), stage + l * kPBytes, at_p, i, kk);
     };
     auto q_frag = [&](const char* stage, int l, int j, int kk) {
-        return frag(std::integral_constant<bool, kQCols>(), std::integral_constant<int, BQ>(), stage + F::kPlanes * kPBytes + l * kQBytes, at_q, j, kk);
+        return frag(QCols(), Pair(), std::integral_constant<int, BQ>(), stage + F::kPlanes * kPBytes + l * kQBytes, at_q, j, kk);
     };
     if (steps > 0) {
         fetch_segment(0);
@@ -613,15 +646,15 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         }
     }
 
-    // ---- lane: output row fr of fragment i, four consecutive q
+    // ---- lane: output row fr of P's fragment i, and of Q's fragments the columns column(j) .. + 3 (paired: of two, eight)
     const T* bias = PRODUCT == kForward && a.bias && !none ? static_cast<const T*>(a.bias) + (int64_t)tl.g * a.n_out : nullptr;
-    const bool whole = n_q % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;  // four results are one 8-byte store
+    auto column = [&](int j) { return q0 + qw + (kPair ? 32 * (j >> 1) + 8 * kg + 4 * (j & 1) : 16 * j + 4 * kg); };
     if (bias)
 #pragma unroll
         for (int j = 0; j < FQ; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int q = q0 + qw + 16 * j + 4 * kg + e;
+                const int q = column(j) + e;
                 const float b = (float)bias[q < n_q ? q : 0];
 #pragma unroll
                 for (int i = 0; i < FP; ++i) acc[i][j][e] += b;
@@ -637,26 +670,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             if (rows_lds[p] < 0) continue;
             at = (int64_t)rows_lds[p] * n_q;
         }
+        if (PRODUCT == kGradWeight && a.chunk_rows) {
 #pragma unroll
-        for (int j = 0; j < FQ; ++j) {
-            const int q = q0 + qw + 16 * j + 4 * kg;
-            const f32x4 v = acc[i][j];
-            if (PRODUCT == kGradWeight && a.chunk_rows) {
-                if (n_q % 4 == 0) {
-                    if (q < n_q) *reinterpret_cast<f32x4*>(a.part + at + q) = v;
-                } else {
+            for (int j = 0; j < FQ; ++j) store_some<float, 4>(a.part + at, column(j), n_q, [&](int e) { return acc[i][j][e]; });
+        } else {
+            constexpr int kOnce = 16 / sizeof(T);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (q + e < n_q) a.part[at + q + e] = v[e];
-                }
-            } else if (whole) {
-                typedef T T4 __attribute__((ext_vector_type(4)));
-                if (q < n_q) *reinterpret_cast<T4*>(static_cast<T*>(a.out) + at + q) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (q + e < n_q) static_cast<T*>(a.out)[at + q + e] = (T)v[e];
-            }
+            for (int j = 0; j < FQ; j += kOnce / 4)
+                store_some<T, kOnce>(static_cast<T*>(a.out) + at, column(j), n_q, [&](int e) { return acc[i][j + (e >> 2)][e & 3]; });
         }
         if (sum_bias) {
             float v = sumb[i] + accb[i];  // of the rows 8 kg .. 8 kg + 7 of every 32
@@ -783,23 +804,9 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
                     }
             }
             if (out_row < 0) continue;
-            constexpr int kOnce = 16 / sizeof(T);  // columns a store takes
-            typedef T Some __attribute__((ext_vector_type(kOnce)));
-            typedef Some Anywhere __attribute__((aligned(sizeof(T))));
+            constexpr int kOnce = 16 / sizeof(T);
 #pragma unroll
-            for (int h = 0; h < 16 / kOnce; ++h) {
-                const int q = column(b, h * (kOnce / 4));
-                Some o;
-#pragma unroll
-                for (int e = 0; e < kOnce; ++e) o[e] = (T)acc[h * (kOnce / 4) + (e >> 2)][e & 3];
-                if (q + kOnce <= width) {
-                    *reinterpret_cast<Anywhere*>(out + q) = o;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kOnce; ++e)
-                        if (q + e < width) out[q + e] = o[e];
-                }
-            }
+            for (int j = 0; j < 4; j += kOnce / 4) store_some<T, kOnce>(out, column(b, j), width, [&](int e) { return acc[j + (e >> 2)][e & 3]; });
         }
     }
 }
