@@ -439,6 +439,9 @@ int mcmc_tft_adamw(mcmc_ctx* ctx, float* P, float* PT, int num_features, const f
 #define MCMC_GROUPED_MAX_ROWS ((int64_t)1 << 30)
 #define MCMC_GROUPED_MAX_DIM (1 << 30)
 #define MCMC_GROUP_ROWS_MAX_GROUPS 4096
+#define MCMC_GROUPED_FORWARD 0     /* the products of mcmc_grouped_linear_* (mcmc_grouped_linear_workspace_bytes) */
+#define MCMC_GROUPED_GRAD_INPUT 1
+#define MCMC_GROUPED_GRAD_WEIGHT 2
 int64_t mcmc_group_rows_workspace_bytes(int64_t rows, int n_groups);
 int mcmc_group_rows(mcmc_ctx* ctx, const void* ids, int id_bytes, int64_t rows, int n_groups, int32_t* order,
                     int32_t* offsets, void* workspace, mcmc_stream_t stream);
@@ -451,18 +454,18 @@ int mcmc_group_rows(mcmc_ctx* ctx, const void* ids, int id_bytes, int64_t rows, 
  *   order   [rows] int32, every row once, or NULL (row r is at position r);  offsets [n_groups + 1] int32, from 0, not
  *           decreasing, at most rows: device memory, e.g. from mcmc_group_rows.  Positions from offsets[n_groups] on are rows of
  *           no group.  Values outside these bounds give wrong results but no access outside the arrays.
- * Pointers need the alignment of their elements only. */
+ *   workspace mcmc_grouped_linear_workspace_bytes(product, ...) bytes of device memory (often 0: NULL is fine), 16-byte aligned,
+ *           contents irrelevant before and after: partial sums, which meet in a fixed order (no atomics, the same bits every time)
+ * Other pointers need the alignment of their elements only. */
+int64_t mcmc_grouped_linear_workspace_bytes(int product, int dtype, int64_t rows, int n_groups, int n_in, int n_out);
 int mcmc_grouped_linear_forward(mcmc_ctx* ctx, int dtype, const void* x, int64_t ld_x, int64_t rows, const int32_t* order,
                                 const int32_t* offsets, int n_groups, int n_in, int n_out, const void* weight,
-                                const void* bias, void* y, mcmc_stream_t stream);
+                                const void* bias, void* y, void* workspace, mcmc_stream_t stream);
 /* dx[r] = weight[g]^T dy[r]; rows of no group: 0.  dy [rows, n_out], ld_dy elements between rows; dx [rows, n_in] dense. */
 int mcmc_grouped_linear_grad_input(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, int64_t rows,
                                    const int32_t* order, const int32_t* offsets, int n_groups, int n_in, int n_out,
-                                   const void* weight, void* dx, mcmc_stream_t stream);
-/* dweight[g] = sum of dy[r] x[r]^T over the rows of g, dbias[g] = sum of dy[r] (dbias may be NULL); groups without rows: 0.
- * Partial sums meet in a fixed order in workspace (mcmc_grouped_linear_workspace_bytes, may be 0; 16-byte aligned): no atomics,
- * the same bits every time. */
-int64_t mcmc_grouped_linear_workspace_bytes(int dtype, int64_t rows, int n_groups, int n_in, int n_out);
+                                   const void* weight, void* dx, void* workspace, mcmc_stream_t stream);
+/* dweight[g] = sum of dy[r] x[r]^T over the rows of g, dbias[g] = sum of dy[r] (dbias may be NULL); groups without rows: 0. */
 int mcmc_grouped_linear_grad_weight(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
                                     int64_t rows, const int32_t* order, const int32_t* offsets, int n_groups, int n_in,
                                     int n_out, void* dweight, void* dbias, void* workspace, mcmc_stream_t stream);

@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("MCMC_LIB_PATH") or os.path.join(_HERE, "lib", "libmcm
 
 DT_F32, DT_BF16, DT_BF16_FAST, DT_F16 = 0, 1, 2, 3
 ACT_NONE, ACT_ELU = 0, 1
+GROUPED_FORWARD, GROUPED_GRAD_INPUT, GROUPED_GRAD_WEIGHT = 0, 1, 2
 NOISE_NONE, NOISE_INJECTED, NOISE_PHILOX = 0, 1, 2
 ABI_VERSION = 22
 
@@ -117,9 +118,9 @@ SIGNATURES = {
                                _stream]),
     "mcmc_group_rows_workspace_bytes": (_i64, [_i64, _i32]),
     "mcmc_group_rows": (_i32, [_ctx_p, _ptr, _i32, _i64, _i32, _ptr, _ptr, _ptr, _stream]),
-    "mcmc_grouped_linear_forward": (_i32, [_ctx_p, _i32, _ptr, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _ptr, _ptr, _ptr, _stream]),
-    "mcmc_grouped_linear_grad_input": (_i32, [_ctx_p, _i32, _ptr, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _ptr, _ptr, _stream]),
-    "mcmc_grouped_linear_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32]),
+    "mcmc_grouped_linear_forward": (_i32, [_ctx_p, _i32, _ptr, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _ptr, _ptr, _ptr, _ptr, _stream]),
+    "mcmc_grouped_linear_grad_input": (_i32, [_ctx_p, _i32, _ptr, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _ptr, _ptr, _ptr, _stream]),
+    "mcmc_grouped_linear_workspace_bytes": (_i64, [_i32, _i32, _i64, _i32, _i32, _i32]),
     "mcmc_grouped_linear_grad_weight": (_i32, [_ctx_p, _i32, _ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _ptr, _ptr, _ptr, _stream]),
     "mcmc_dropout_forward": (_i32, [_ctx_p, _i32, _i32, _ptr, _i64, _i64, _i64, _u64, _ptr, _f32, _i64, _i64, _i64, _ptr, _i64, _stream]),
     "mcmc_dropout_backward": (_i32, [_ctx_p, _i32, _i32, _ptr, _i64, _ptr, _i64, _i64, _i64, _u64, _ptr, _f32, _i64, _i64, _i64, _ptr, _i64, _stream]),

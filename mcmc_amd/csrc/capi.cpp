@@ -752,14 +752,22 @@ static int check_grouped_dims(int64_t rows, int n_groups, int n_in, int n_out) {
     return MCMC_OK;
 }
 
-int64_t mcmc_grouped_linear_workspace_bytes(int dtype, int64_t rows, int n_groups, int n_in, int n_out) {
+int64_t mcmc_grouped_linear_workspace_bytes(int product, int dtype, int64_t rows, int n_groups, int n_in, int n_out) {
+    MCMC_REQUIRE(product >= MCMC_GROUPED_FORWARD && product <= MCMC_GROUPED_GRAD_WEIGHT, "product must be one of MCMC_GROUPED_* (got %d)", product);
     if (int rc = check_operand_dtype(dtype)) return rc;
     if (int rc = check_grouped_dims(rows, n_groups, n_in, n_out)) return rc;
-    return grouped_linear_workspace_bytes(rows, n_groups, n_in, n_out);
+    return grouped_linear_workspace_bytes(product, dtype, rows, n_groups, n_in, n_out);
+}
+
+static int check_grouped_workspace(int product, int dtype, int64_t rows, int n_groups, int n_in, int n_out, const void* workspace) {
+    if (grouped_linear_workspace_bytes(product, dtype, rows, n_groups, n_in, n_out) > 0)
+        MCMC_REQUIRE(workspace && aligned16(workspace), "workspace must be 16-byte aligned device memory (mcmc_grouped_linear_workspace_bytes)");
+    return MCMC_OK;
 }
 
 int mcmc_grouped_linear_forward(mcmc_ctx* ctx, int dtype, const void* x, int64_t ld_x, int64_t rows, const int32_t* order, const int32_t* offsets,
-                                int n_groups, int n_in, int n_out, const void* weight, const void* bias, void* y, mcmc_stream_t stream) {
+                                int n_groups, int n_in, int n_out, const void* weight, const void* bias, void* y, void* workspace,
+                                mcmc_stream_t stream) {
     if (int rc = check_ctx(ctx)) return rc;
     if (int rc = check_operand_dtype(dtype)) return rc;
     if (int rc = check_grouped_dims(rows, n_groups, n_in, n_out)) return rc;
@@ -768,11 +776,13 @@ int mcmc_grouped_linear_forward(mcmc_ctx* ctx, int dtype, const void* x, int64_t
     MCMC_REQUIRE(x && offsets && weight && y, "x / offsets / weight / y is NULL");
     MCMC_REQUIRE(aligned_for(dtype, x) && aligned_for(dtype, weight) && aligned_for(dtype, bias) && aligned_for(dtype, y),
                  "x, weight, bias and y must be aligned to their elements");
-    return launch_grouped_linear_forward(dtype, x, ld_x, rows, order, offsets, n_groups, n_in, n_out, weight, bias, y, (hipStream_t)stream);
+    if (int rc = check_grouped_workspace(MCMC_GROUPED_FORWARD, dtype, rows, n_groups, n_in, n_out, workspace)) return rc;
+    return launch_grouped_linear_forward(dtype, x, ld_x, rows, order, offsets, n_groups, n_in, n_out, weight, bias, y, workspace, (hipStream_t)stream);
 }
 
 int mcmc_grouped_linear_grad_input(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, int64_t rows, const int32_t* order,
-                                   const int32_t* offsets, int n_groups, int n_in, int n_out, const void* weight, void* dx, mcmc_stream_t stream) {
+                                   const int32_t* offsets, int n_groups, int n_in, int n_out, const void* weight, void* dx, void* workspace,
+                                   mcmc_stream_t stream) {
     if (int rc = check_ctx(ctx)) return rc;
     if (int rc = check_operand_dtype(dtype)) return rc;
     if (int rc = check_grouped_dims(rows, n_groups, n_in, n_out)) return rc;
@@ -780,7 +790,8 @@ int mcmc_grouped_linear_grad_input(mcmc_ctx* ctx, int dtype, const void* dy, int
     if (rows == 0) return MCMC_OK;
     MCMC_REQUIRE(dy && offsets && weight && dx, "dy / offsets / weight / dx is NULL");
     MCMC_REQUIRE(aligned_for(dtype, dy) && aligned_for(dtype, weight) && aligned_for(dtype, dx), "dy, weight and dx must be aligned to their elements");
-    return launch_grouped_linear_grad_input(dtype, dy, ld_dy, rows, order, offsets, n_groups, n_in, n_out, weight, dx, (hipStream_t)stream);
+    if (int rc = check_grouped_workspace(MCMC_GROUPED_GRAD_INPUT, dtype, rows, n_groups, n_in, n_out, workspace)) return rc;
+    return launch_grouped_linear_grad_input(dtype, dy, ld_dy, rows, order, offsets, n_groups, n_in, n_out, weight, dx, workspace, (hipStream_t)stream);
 }
 
 int mcmc_grouped_linear_grad_weight(mcmc_ctx* ctx, int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows,
@@ -794,8 +805,7 @@ int mcmc_grouped_linear_grad_weight(mcmc_ctx* ctx, int dtype, const void* dy, in
     MCMC_REQUIRE(rows == 0 || (dy && x), "dy / x is NULL");
     MCMC_REQUIRE(aligned_for(dtype, dy) && aligned_for(dtype, x) && aligned_for(dtype, dweight) && aligned_for(dtype, dbias),
                  "dy, x, dweight and dbias must be aligned to their elements");
-    if (grouped_linear_workspace_bytes(rows, n_groups, n_in, n_out) > 0)
-        MCMC_REQUIRE(workspace && aligned16(workspace), "workspace must be 16-byte aligned device memory (mcmc_grouped_linear_workspace_bytes)");
+    if (int rc = check_grouped_workspace(MCMC_GROUPED_GRAD_WEIGHT, dtype, rows, n_groups, n_in, n_out, workspace)) return rc;
     return launch_grouped_linear_grad_weight(dtype, dy, ld_dy, x, ld_x, rows, order, offsets, n_groups, n_in, n_out, dweight, dbias, workspace,
                                              (hipStream_t)stream);
 }

@@ -154,10 +154,10 @@ int launch_flat_update(float* param, int64_t n, const float* dP, int B, float* g
 int64_t group_rows_workspace_bytes(int64_t rows, int G);
 int launch_group_rows(const void* ids, int id_bytes, int64_t rows, int G, int* order, int* offsets, void* ws, hipStream_t s);
 int launch_grouped_linear_forward(int dtype, const void* x, int64_t ld_x, int64_t rows, const int* order, const int* offsets, int G, int n_in,
-                                  int n_out, const void* weight, const void* bias, void* y, hipStream_t s);
+                                  int n_out, const void* weight, const void* bias, void* y, void* ws, hipStream_t s);
 int launch_grouped_linear_grad_input(int dtype, const void* dy, int64_t ld_dy, int64_t rows, const int* order, const int* offsets, int G, int n_in,
-                                     int n_out, const void* weight, void* dx, hipStream_t s);
-int64_t grouped_linear_workspace_bytes(int64_t rows, int G, int n_in, int n_out);
+                                     int n_out, const void* weight, void* dx, void* ws, hipStream_t s);
+int64_t grouped_linear_workspace_bytes(int product, int dtype, int64_t rows, int G, int n_in, int n_out);
 int launch_grouped_linear_grad_weight(int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows, const int* order,
                                       const int* offsets, int G, int n_in, int n_out, void* dweight, void* dbias, void* ws, hipStream_t s);
 // backward: out = dx from dy (and x, the forward's input, with an activation)

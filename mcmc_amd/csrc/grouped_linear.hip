@@ -24,7 +24,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-enum Product { kForward, kGradInput, kGradWeight };
+enum Product { kForward = MCMC_GROUPED_FORWARD, kGradInput = MCMC_GROUPED_GRAD_INPUT, kGradWeight = MCMC_GROUPED_GRAD_WEIGHT };
 
 struct Args {
     const void* p;  // x (forward), dy (dx, dW): rows of ld_p elements
@@ -32,13 +32,15 @@ struct Args {
     const void* bias;
     void* out;      // y, dx, dW
     void* dbias;
-    float* part;    // dW in chunks: [chunk][n_out][n_in] then [chunk][n_out]
+    float* part;    // partial sums.  dW in chunks: [chunk][n_out][n_in] then [chunk][n_out]; a split contraction: [split][rows][n_q]
     const int* order;
     const int* offsets;
     int64_t ld_p, ld_q, rows;
     int G, n_in, n_out;
     int chunk_rows;  // dW: rows per partial sum (0: a group is one sum, written to `out`)
     int chunks;      // dW: partial sums there is room for
+    int splits;      // forward, dx: parts of the contraction, each a workgroup's
+    int split_c;     // contraction elements of a part
 };
 
 // ---- matrix instructions: 16 x 16 outputs, 32 contraction elements ---------------------------------------------------------
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     // together share both operands
     constexpr int kBand = 8;
     int64_t id;
-    int run = 0, p0 = 0, q0;
+    int run = 0, split = 0, p0 = 0, q0;
     Tile tl;
     if (PRODUCT == kGradWeight) {
         const int p_tiles = (a.n_out + BP - 1) / BP, per_run = p_tiles * q_tiles;
@@ -348,9 +350,10 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         }
     } else {
         const Runs all = count_runs(a.offsets, a.G, rows, BP, a.G);
-        const int64_t tiles = all.total;
-        if ((int64_t)blockIdx.x >= tiles * q_tiles) return;
-        id = xcd_order(blockIdx.x, tiles * q_tiles);
+        const int64_t tiles = all.total, block = blockIdx.x / a.splits;
+        if (block >= tiles * q_tiles) return;
+        split = (int)(blockIdx.x % a.splits);
+        id = xcd_order(block, tiles * q_tiles);
         const int64_t band = id / (kBand * q_tiles), left = tiles - band * kBand, high = left < kBand ? left : kBand;
         const int64_t at = id - band * kBand * q_tiles;
         tl = nth_run(a.offsets, a.G, rows, BP, all, (int)(band * kBand + at % high));
@@ -359,10 +362,16 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         __syncthreads();
     }
     const bool none = PRODUCT != kGradWeight && tl.g == a.G;
-    const int n_c = none ? 0 : PRODUCT == kForward ? a.n_in : PRODUCT == kGradInput ? a.n_out : tl.last - tl.first;
+    int n_c = none ? 0 : PRODUCT == kForward ? a.n_in : PRODUCT == kGradInput ? a.n_out : tl.last - tl.first;
+    const T* P = static_cast<const T*>(a.p);
+    const T* Q = static_cast<const T*>(a.q) + (PRODUCT != kGradWeight && !none ? (int64_t)tl.g * a.n_in * a.n_out : 0);
+    if (PRODUCT != kGradWeight && a.splits > 1) {  // this workgroup's part of the contraction
+        const int c = split * a.split_c;
+        n_c = n_c - c < a.split_c ? (n_c > c ? n_c - c : 0) : a.split_c;
+        P += c;
+        Q += PRODUCT == kForward ? c : (int64_t)c * a.ld_q;
+    }
     const int steps = (n_c + BC - 1) / BC;
-    const T* const P = static_cast<const T*>(a.p);
-    const T* const Q = static_cast<const T*>(a.q) + (PRODUCT != kGradWeight && !none ? (int64_t)tl.g * a.n_in * a.n_out : 0);
     const T* const zeros = reinterpret_cast<const T*>(kZeros);
 
     // ---- where this lane's pieces come from.  "rows": the chunk's address at step 0, kept.  "columns": row of the tile and first column,
@@ -647,7 +656,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     }
 
     // ---- lane: output row fr of P's fragment i, and of Q's fragments the columns column(j) .. + 3 (paired: of two, eight)
-    const T* bias = PRODUCT == kForward && a.bias && !none ? static_cast<const T*>(a.bias) + (int64_t)tl.g * a.n_out : nullptr;
+    const T* bias = PRODUCT == kForward && a.bias && !none && split == 0 ? static_cast<const T*>(a.bias) + (int64_t)tl.g * a.n_out : nullptr;
     auto column = [&](int j) { return q0 + qw + (kPair ? 32 * (j >> 1) + 8 * kg + 4 * (j & 1) : 16 * j + 4 * kg); };
     if (bias)
 #pragma unroll
@@ -673,6 +682,10 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         if (PRODUCT == kGradWeight && a.chunk_rows) {
 #pragma unroll
             for (int j = 0; j < FQ; ++j) store_some<float, 4>(a.part + at, column(j), n_q, [&](int e) { return acc[i][j][e]; });
+        } else if (PRODUCT != kGradWeight && a.splits > 1) {
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+                store_some<float, 4>(a.part + ((int64_t)split * rows + rows_lds[p]) * n_q, column(j), n_q, [&](int e) { return acc[i][j][e]; });
         } else {
             constexpr int kOnce = 16 / sizeof(T);
 #pragma unroll
@@ -928,6 +941,16 @@ __global__ __launch_bounds__(kThreads) void grouped_sum_kernel(Args a) {
     else static_cast<T*>(a.dbias)[(int64_t)g * a.n_out + (i - n)] = (T)s;
 }
 
+// y or dx = the sum of a split contraction's parts, in their order
+template <typename T>
+__global__ __launch_bounds__(kThreads) void grouped_join_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= n) return;
+    float s = part[i];
+    for (int k = 1; k < splits; ++k) s += part[k * n + i];
+    out[i] = (T)s;
+}
+
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 struct Shape {
@@ -1015,21 +1038,50 @@ int launch_strip(const Args& a, int q_tile, hipStream_t s) {
     return MCMC_EINVAL;  // strip_q_tile takes no fp32 contraction beyond 128
 }
 
+// Parts of a long contraction (forward, dx) where the output has too few tiles to fill the chip: a step of one workgroup waits for
+// memory, so 64 of them take 30 us on however few tiles.  4096 -> 512, 8 rows in 2 groups: 30 us whole, 15 in parts with the launch
+// that joins them; up to 1,024 elements the joining costs more than the steps (512 -> 512, 1,000 rows: 10 us whole, 16 in parts).
+struct Split {
+    int parts, c;
+};
 template <typename T>
-int launch(int product, const Args& a, hipStream_t s) {
+Split split_of(int product, int64_t rows, int G, int n_in, int n_out) {
+    const int n_c = product == kForward ? n_in : n_out, n_q = product == kForward ? n_out : n_in;
+    const int64_t tiles = (rows / 128 + (G + 1 < rows ? G + 1 : rows)) * ceil_div(n_q, 128);
+    if (product == kGradWeight || rows == 0 || strip_q_tile<T>(n_c, n_q) || tiles >= 256 || n_c < (sizeof(T) == 4 ? 1024 : 1536)) return Split{1, n_c};
+    int64_t parts = 512 / tiles;
+    parts = parts > 16 ? 16 : parts;
+    parts = parts > n_c / 256 ? n_c / 256 : parts;
+    const int c = ceil_div(ceil_div(n_c, parts), 64) * 64;
+    return Split{ceil_div(n_c, c), c};
+}
+
+template <typename T>
+int launch(int product, Args a, hipStream_t s) {
     const int n_q = product == kForward ? a.n_out : a.n_in;
     if (product != kGradWeight) {
         if (const int q_tile = strip_q_tile<T>(product == kForward ? a.n_in : a.n_out, n_q))
             return product == kForward ? launch_strip<T, kForward>(a, q_tile, s) : launch_strip<T, kGradInput>(a, q_tile, s);
     }
+    const Split split = split_of<T>(product, a.rows, a.G, a.n_in, a.n_out);
+    a.splits = split.parts;
+    a.split_c = split.c;
     const bool dma = sizeof(T) == 2 && whole_chunks(product, a);
     const Shape sh = shape_of(product, dma, a.rows, a.G, a.n_in, a.n_out);
     const int64_t runs = product == kGradWeight ? (int64_t)ceil_div(a.n_out, sh.bp) * (a.chunk_rows ? a.chunks : a.G)
-                                                : a.rows / sh.bp + (a.G + 1 < a.rows ? a.G + 1 : a.rows);
+                                                : (a.rows / sh.bp + (a.G + 1 < a.rows ? a.G + 1 : a.rows)) * a.splits;
     const int64_t blocks = runs * ceil_div(n_q, sh.bq);
     if (int rc = check_grid(blocks)) return rc;
-    if (product == kForward) return launch_product<T, kForward>(a, sh, dma, (unsigned)blocks, s);
-    if (product == kGradInput) return launch_product<T, kGradInput>(a, sh, dma, (unsigned)blocks, s);
+    if (product != kGradWeight) {
+        if (int rc = product == kForward ? launch_product<T, kForward>(a, sh, dma, (unsigned)blocks, s)
+                                         : launch_product<T, kGradInput>(a, sh, dma, (unsigned)blocks, s))
+            return rc;
+        if (a.splits == 1) return MCMC_OK;
+        const int64_t n = a.rows * n_q, joins = (n + kThreads - 1) / kThreads;
+        if (int rc = check_grid(joins)) return rc;
+        grouped_join_kernel<T><<<(unsigned)joins, kThreads, 0, s>>>(a.part, a.splits, n, static_cast<T*>(a.out));
+        return check_launch("grouped_join_kernel");
+    }
     const bool thin_out = a.n_out <= kThinMost;
     if (thin_out || a.n_in < kThinMost) {
         const int64_t thin = (int64_t)ceil_div(thin_out ? a.n_in : a.n_out, kThinCols) * (a.chunk_rows ? a.chunks : a.G);
@@ -1059,18 +1111,24 @@ int launch_typed(int dtype, int product, const Args& a, hipStream_t s) {
 }  // namespace
 
 int launch_grouped_linear_forward(int dtype, const void* x, int64_t ld_x, int64_t rows, const int* order, const int* offsets, int G, int n_in,
-                                  int n_out, const void* weight, const void* bias, void* y, hipStream_t s) {
-    return launch_typed(dtype, kForward, Args{x, weight, bias, y, nullptr, nullptr, order, offsets, ld_x, n_in, rows, G, n_in, n_out, 0, 0}, s);
+                                  int n_out, const void* weight, const void* bias, void* y, void* ws, hipStream_t s) {
+    return launch_typed(dtype, kForward,
+                        Args{x, weight, bias, y, nullptr, static_cast<float*>(ws), order, offsets, ld_x, n_in, rows, G, n_in, n_out, 0, 0, 1, 0}, s);
 }
 
 int launch_grouped_linear_grad_input(int dtype, const void* dy, int64_t ld_dy, int64_t rows, const int* order, const int* offsets, int G, int n_in,
-                                     int n_out, const void* weight, void* dx, hipStream_t s) {
-    return launch_typed(dtype, kGradInput, Args{dy, weight, nullptr, dx, nullptr, nullptr, order, offsets, ld_dy, n_in, rows, G, n_in, n_out, 0, 0}, s);
+                                     int n_out, const void* weight, void* dx, void* ws, hipStream_t s) {
+    return launch_typed(dtype, kGradInput,
+                        Args{dy, weight, nullptr, dx, nullptr, static_cast<float*>(ws), order, offsets, ld_dy, n_in, rows, G, n_in, n_out, 0, 0, 1, 0}, s);
 }
 
-int64_t grouped_linear_workspace_bytes(int64_t rows, int G, int n_in, int n_out) {
-    const int per = chunk_rows_of(rows, G, n_in, n_out);
-    return per ? (int64_t)chunks_of(rows, G, per) * ((int64_t)n_in + 1) * n_out * 4 : 0;
+int64_t grouped_linear_workspace_bytes(int product, int dtype, int64_t rows, int G, int n_in, int n_out) {
+    if (product == kGradWeight) {
+        const int per = chunk_rows_of(rows, G, n_in, n_out);
+        return per ? (int64_t)chunks_of(rows, G, per) * ((int64_t)n_in + 1) * n_out * 4 : 0;
+    }
+    const Split split = dtype == MCMC_DT_F32 ? split_of<float>(product, rows, G, n_in, n_out) : split_of<__bf16>(product, rows, G, n_in, n_out);
+    return split.parts > 1 ? (int64_t)split.parts * rows * (product == kForward ? n_out : n_in) * 4 : 0;
 }
 
 int launch_grouped_linear_grad_weight(int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows, const int* order,
@@ -1078,7 +1136,7 @@ int launch_grouped_linear_grad_weight(int dtype, const void* dy, int64_t ld_dy, 
     const int per = chunk_rows_of(rows, G, n_in, n_out);
     return launch_typed(dtype, kGradWeight,
                         Args{dy, x, nullptr, dweight, dbias, static_cast<float*>(ws), order, offsets, ld_dy, ld_x, rows, G, n_in, n_out, per,
-                             per ? chunks_of(rows, G, per) : 0},
+                             per ? chunks_of(rows, G, per) : 0, 1, 0},
                         s);
 }
 

@@ -130,26 +130,32 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
 
 
 # ---- grouped_linear ---------------------------------------------------------------------------------------------------------
+def _workspace(eng: Engine, product: int, dt: int, R: int, G: int, K: int, N: int, dev) -> Optional[torch.Tensor]:
+    n = _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(product, dt, R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
 def _forward(eng: Engine, x, weight, bias, order, offsets):
     (R, K), (G, N, _) = x.shape, weight.shape
-    y = torch.empty((R, N), dtype=x.dtype, device=x.device)
-    _lib.check(eng.lib.mcmc_grouped_linear_forward(eng.ctx.handle, _DT[x.dtype], x.data_ptr(), x.stride(0), R, _ptr(order), offsets.data_ptr(), G, K, N,
-                                                   weight.data_ptr(), _ptr(bias), y.data_ptr(), _stream(eng)), "mcmc_grouped_linear_forward")
+    dt, y = _DT[x.dtype], torch.empty((R, N), dtype=x.dtype, device=x.device)
+    ws = _workspace(eng, _lib.GROUPED_FORWARD, dt, R, G, K, N, x.device)
+    _lib.check(eng.lib.mcmc_grouped_linear_forward(eng.ctx.handle, dt, x.data_ptr(), x.stride(0), R, _ptr(order), offsets.data_ptr(), G, K, N,
+                                                   weight.data_ptr(), _ptr(bias), y.data_ptr(), _ptr(ws), _stream(eng)), "mcmc_grouped_linear_forward")
     return y
 
 
 def _grad_input(eng: Engine, dy, weight, order, offsets):
     R, (G, N, K) = dy.shape[0], weight.shape
-    dx = torch.empty((R, K), dtype=dy.dtype, device=dy.device)
-    _lib.check(eng.lib.mcmc_grouped_linear_grad_input(eng.ctx.handle, _DT[dy.dtype], dy.data_ptr(), dy.stride(0), R, _ptr(order), offsets.data_ptr(), G, K, N,
-                                                      weight.data_ptr(), dx.data_ptr(), _stream(eng)), "mcmc_grouped_linear_grad_input")
+    dt, dx = _DT[dy.dtype], torch.empty((R, K), dtype=dy.dtype, device=dy.device)
+    ws = _workspace(eng, _lib.GROUPED_GRAD_INPUT, dt, R, G, K, N, dy.device)
+    _lib.check(eng.lib.mcmc_grouped_linear_grad_input(eng.ctx.handle, dt, dy.data_ptr(), dy.stride(0), R, _ptr(order), offsets.data_ptr(), G, K, N,
+                                                      weight.data_ptr(), dx.data_ptr(), _ptr(ws), _stream(eng)), "mcmc_grouped_linear_grad_input")
     return dx
 
 
 def _grad_weight(eng: Engine, dy, x, order, offsets, G: int, want_bias: bool):
     (R, K), N, dt, dev = x.shape, dy.shape[1], _DT[x.dtype], x.device
-    ws_bytes = _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(dt, R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    ws = _workspace(eng, _lib.GROUPED_GRAD_WEIGHT, dt, R, G, K, N, dev)
     dw = torch.empty((G, N, K), dtype=x.dtype, device=dev)
     db = torch.empty((G, N), dtype=x.dtype, device=dev) if want_bias else None
     _lib.check(eng.lib.mcmc_grouped_linear_grad_weight(eng.ctx.handle, dt, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), R, _ptr(order),

@@ -332,12 +332,12 @@ int main() {
                 EXPECT(w >= 0, ok);
                 if (ok && rows > 8192) EXPECT(w >= (int64_t)4 * (groups + 1), 1);
                 const bool okl = rows >= 0 && rows < big && groups >= 1;
-                for (int n : {0, 1, 64, 4096}) EXPECT(mcmc_grouped_linear_workspace_bytes(MCMC_DT_F16, rows, groups, n, 64) >= 0, okl && n >= 1);
+                for (int n : {0, 1, 64, 4096}) EXPECT(mcmc_grouped_linear_workspace_bytes((groups + 3) % 3, MCMC_DT_F16, rows, groups, n, 64) >= 0, okl && n >= 1);
             }
-        EXPECT_EINVAL(mcmc_grouped_linear_workspace_bytes(0, 4, 1, (1 << 30) + 1, 1));
+        EXPECT_EINVAL(mcmc_grouped_linear_workspace_bytes(2, 0, 4, 1, (1 << 30) + 1, 1));
         EXPECT(mcmc_group_rows(z, i32, 4, 4, 2, i32, i32, nullptr, s), MCMC_ESTATE);
-        EXPECT(mcmc_grouped_linear_forward(z, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, f, s), MCMC_ESTATE);
-        EXPECT(mcmc_grouped_linear_grad_input(z, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, s), MCMC_ESTATE);
+        EXPECT(mcmc_grouped_linear_forward(z, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, f, v, s), MCMC_ESTATE);
+        EXPECT(mcmc_grouped_linear_grad_input(z, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s), MCMC_ESTATE);
         EXPECT(mcmc_grouped_linear_grad_weight(z, 0, f, 4, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s), MCMC_ESTATE);
         EXPECT(mcmc_dropout_forward(z, 0, 0, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s), MCMC_ESTATE);
         EXPECT(mcmc_dropout_backward(z, 0, 0, f, 4, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s), MCMC_ESTATE);
@@ -353,31 +353,38 @@ int main() {
         EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, 100000, 2, i32, i32, nullptr, s));      // workspace
         EXPECT_EINVAL(mcmc_group_rows(c, i32, 4, 100000, 2, i32, i32, f_odd, s));
         for (int dt : {-1, MCMC_DT_BF16_FAST, 4}) {
-            EXPECT_EINVAL(mcmc_grouped_linear_forward(c, dt, f, 4, 4, i32, i32, 2, 4, 4, f, f, f, s));
-            EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, dt, f, 4, 4, i32, i32, 2, 4, 4, f, f, s));
+            EXPECT_EINVAL(mcmc_grouped_linear_forward(c, dt, f, 4, 4, i32, i32, 2, 4, 4, f, f, f, v, s));
+            EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, dt, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s));
             EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, dt, f, 4, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s));
             EXPECT_EINVAL(mcmc_dropout_forward(c, dt, 0, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
             EXPECT_EINVAL(mcmc_dropout_backward(c, dt, 0, f, 4, f, 4, 4, 4, 1, nullptr, 0.1f, 0, 0, 0, f, 4, s));
         }
-        EXPECT(mcmc_grouped_linear_forward(c, 0, nullptr, 4, 0, nullptr, nullptr, 2, 4, 4, nullptr, nullptr, nullptr, s), MCMC_OK);
-        EXPECT(mcmc_grouped_linear_grad_input(c, 1, nullptr, 4, 0, nullptr, nullptr, 2, 4, 4, nullptr, nullptr, s), MCMC_OK);
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, -1, 4, i32, i32, 2, 4, 4, f, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, big, i32, i32, 2, 4, 4, f, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 0, 4, 4, f, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 0, 4, f, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, nullptr, 2, 4, 4, f, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, nullptr, 4, 4, i32, i32, 2, 4, 4, f, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, nullptr, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 1, u8_odd, 4, 4, i32, i32, 2, 4, 4, f, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, -4, 4, i32, i32, 2, 4, 4, f, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, s));
-        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, 4, 4, i32, i32, 2, 4, 4, f, u8_odd, s));
+        EXPECT(mcmc_grouped_linear_forward(c, 0, nullptr, 4, 0, nullptr, nullptr, 2, 4, 4, nullptr, nullptr, nullptr, v, s), MCMC_OK);
+        EXPECT(mcmc_grouped_linear_grad_input(c, 1, nullptr, 4, 0, nullptr, nullptr, 2, 4, 4, nullptr, nullptr, v, s), MCMC_OK);
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, -1, 4, i32, i32, 2, 4, 4, f, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, big, i32, i32, 2, 4, 4, f, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 0, 4, 4, f, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 0, 4, f, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, nullptr, 2, 4, 4, f, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, nullptr, 4, 4, i32, i32, 2, 4, 4, f, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 0, f, 4, 4, i32, i32, 2, 4, 4, f, f, nullptr, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 1, u8_odd, 4, 4, i32, i32, 2, 4, 4, f, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, -4, 4, i32, i32, 2, 4, 4, f, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, v, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 1, f, 4, 4, i32, i32, 2, 4, 4, f, u8_odd, v, s));
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 4, f, -4, 4, i32, i32, 2, 4, 4, f, f, v, s));
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 4, f, 4, 0, i32, nullptr, 2, 4, 4, f, f, v, s));  // dweight is written for 0 rows too
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 4, f, 4, 4, i32, i32, 2, 4, 4, nullptr, f, v, s));
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, nullptr, 4, f, 4, 4, i32, i32, 2, 4, 4, f, f, v, s));
-        EXPECT(mcmc_grouped_linear_workspace_bytes(1, 1000000, 2, 64, 64) > 0, 1);
+        EXPECT(mcmc_grouped_linear_workspace_bytes(2, 1, 1000000, 2, 64, 64) > 0, 1);
+        for (int product : {-1, 3}) EXPECT_EINVAL(mcmc_grouped_linear_workspace_bytes(product, 1, 4, 2, 4, 4));
+        for (int dt : {-1, 2, 4}) EXPECT_EINVAL(mcmc_grouped_linear_workspace_bytes(0, dt, 4, 2, 4, 4));
+        EXPECT(mcmc_grouped_linear_workspace_bytes(0, 1, 8, 2, 4096, 512) > 0, 1);       // a long contraction on few tiles is split
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 1, f, 4096, 8, i32, i32, 2, 4096, 512, f, f, f, nullptr, s));
+        EXPECT_EINVAL(mcmc_grouped_linear_forward(c, 1, f, 4096, 8, i32, i32, 2, 4096, 512, f, f, f, f_odd, s));
+        EXPECT(mcmc_grouped_linear_workspace_bytes(1, 0, 8, 2, 512, 4096) > 0, 1);
+        EXPECT_EINVAL(mcmc_grouped_linear_grad_input(c, 0, f, 4096, 8, i32, i32, 2, 512, 4096, f, f, nullptr, s));
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 64, f, 64, 1000000, i32, i32, 2, 64, 64, f, f, nullptr, s));
         EXPECT_EINVAL(mcmc_grouped_linear_grad_weight(c, 1, f, 64, f, 64, 1000000, i32, i32, 2, 64, 64, f, f, f_odd, s));
         EXPECT(mcmc_dropout_forward(c, 0, 1, nullptr, 4, 0, 4, 1, nullptr, 0.1f, 0, 0, 0, nullptr, 4, s), MCMC_OK);

@@ -583,3 +583,16 @@ def test_gradients_of_gradients_are_refused():
         assert torch.equal(first.detach(), plain)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             first.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", [(8, 2, 4096, 512), (15, 64, 11, 2772), (5, 2, 2193, 10), (300, 9, 3, 3634), (1, 1, 4096, 4096), (130, 1, 1000, 1111)])
+def test_long_contractions_on_few_tiles(R, G, K, N, dtype):
+    """Contractions split over workgroups, whose partial sums are joined afterwards; rows of no group are zero in every part."""
+    for ordered, stray in ((False, 0.2 if R > 4 else 0.0), (True, 0.0)):
+        x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, 700, ordered, stray)
+        got = run_linear(x, w, b, dy, groups)
+        ref, mag = linear_reference(x, w, b, dy, ids)
+        for n in ref:
+            check(got[n], ref[n], mag[n] * U, n)
+        assert not got["y"][ids < 0].any() and not got["dx"][ids < 0].any()
