@@ -713,7 +713,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 // 16 j + m.  16-bit: fragments 2 h and 2 h + 1 hold columns 32 h + 8 (m >> 2) + 4 (j & 1) + (m & 3), so that two of them are eight
 // consecutive columns.  Either way a lane stores 16 bytes at a time and the four lanes of a row 64 consecutive bytes.
 constexpr int kStripWaves = 8;
-constexpr int kStripLds = 64 * 1024;  // weights of a workgroup: two workgroups a CU
+// LDS for a workgroup's weights: two workgroups a CU; fp32, whose registers allow one, most of it
+template <typename T>
+constexpr int strip_lds() { return sizeof(T) == 4 ? 96 * 1024 : 64 * 1024; }
 
 template <typename T, int PRODUCT, int NC>
 __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grouped_strip_kernel(Args a, int q_tile, int run_rows) {
@@ -757,54 +759,70 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
     infinite = __syncthreads_or(infinite);
 
     auto row_of = [&](int first) { return first + fr < tl.last ? row_at(a, first + fr) : -1; };
+    auto load_one = [&](int row, int k) {
+        const T* const at = P + (int64_t)(row < 0 ? 0 : row) * a.ld_p + 8 * kg + 32 * k;
+        const int n = row < 0 || none ? 0 : n_c - 8 * kg - 32 * k;
+        return n_c % 8 == 0 ? load_eight(at, n) : load_through(at, n, row + 1 < rows && 32 * k + 8 * kg + 8 <= a.ld_p + n_c);
+    };
     auto load_rows = [&](int row, Piece<T> (&u)[NC]) {
-        const T* const at = P + (int64_t)(row < 0 ? 0 : row) * a.ld_p + 8 * kg;
-        const int n = row < 0 || none ? 0 : n_c - 8 * kg;
         if (n_c % 8 == 0) {
 #pragma unroll
-            for (int k = 0; k < NC; ++k) u[k] = load_eight(at + 32 * k, n - 32 * k);
+            for (int k = 0; k < NC; ++k) u[k] = load_one(row, k);
         } else {
 #pragma unroll
-            for (int k = 0; k < NC; ++k) u[k] = load_through(at + 32 * k, n - 32 * k, row + 1 < rows && 32 * k + 8 * kg + 8 <= a.ld_p + n_c);
+            for (int k = 0; k < NC; ++k) u[k] = load_one(row, k);
         }
     };
+    auto column = [&](int b, int j) { return 64 * b + (sizeof(T) == 4 ? 16 * j + 4 * kg : 32 * (j >> 1) + 8 * kg + 4 * (j & 1)); };
     constexpr int kStep = 16 * kStripWaves;
     int first = tl.first + 16 * wave;
     int row = row_of(first), row_next = row_of(first + kStep);
     Piece<T> u[NC];
     load_rows(row, u);
     for (; first < tl.last; first += kStep) {
-        V p[PL][NC];
-        bool bad = infinite;
-#pragma unroll
-        for (int k = 0; k < NC; ++k) {
-            char piece[PL * 16];
-            store_piece(piece, 16, u[k], bad);
-#pragma unroll
-            for (int l = 0; l < PL; ++l) __builtin_memcpy(&p[l][k], piece + 16 * l, 16);
-        }
         const int out_row = row;
+        const bool more = first + kStep < tl.last;
         row = row_next;
-        if (first + kStep < tl.last) {
-            load_rows(row, u);
-            row_next = row_of(first + 2 * kStep);
-        }
         T* const out = static_cast<T*>(a.out) + (int64_t)(out_row < 0 ? 0 : out_row) * n_q + q0;
-        auto column = [&](int b, int j) { return 64 * b + (sizeof(T) == 4 ? 16 * j + 4 * kg : 32 * (j >> 1) + 8 * kg + 4 * (j & 1)); };
+        V p[sizeof(T) == 4 ? 1 : NC];
+        bool bad = infinite;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int k = 0; k < NC; ++k) __builtin_memcpy(&p[k], u[k].v, 16);
+            if (more) load_rows(row, u);
+        }
+        if (more) row_next = row_of(first + 2 * kStep);
         for (int b = 0; b < blocks; ++b) {
             f32x4 acc[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j] = *reinterpret_cast<const f32x4*>(bias + column(b, j));
             const char* w = smem + (b * 4 * NC * 64 + lane) * 16;
 #pragma unroll
-            for (int l = PL - 1; l >= 0; --l)  // small products first, as in the tile kernel
+            for (int k = 0; k < NC; ++k) {
+                V q[PL];
+                if constexpr (sizeof(T) == 2) {
+                    q[0] = p[k];
+                } else {  // split where it is used (behind an empty asm statement): the planes of all k would not fit the registers
 #pragma unroll
-                for (int m = PL - 1 - l; m >= 0; --m)
+                    for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(u[k].v[e]));
+                    char planes[PL * 16];
+                    store_piece(planes, 16, u[k], bad);
+                    if (b + 1 == blocks && more) {
+                        int next = row;
+                        asm volatile("" : "+v"(next));
+                        u[k] = load_one(next, k);
+                    }
 #pragma unroll
-                    for (int k = 0; k < NC; ++k)
+                    for (int l = 0; l < PL; ++l) __builtin_memcpy(&q[l], planes + 16 * l, 16);
+                }
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            acc[j] = F::mfma(*reinterpret_cast<const V*>(w + m * plane_bytes + (j * NC + k) * 1024), p[l][k], acc[j]);
+                for (int l = PL - 1; l >= 0; --l)  // small products first, as in the tile kernel
+#pragma unroll
+                    for (int m = PL - 1 - l; m >= 0; --m)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[j] = F::mfma(*reinterpret_cast<const V*>(w + m * plane_bytes + (j * NC + k) * 1024), q[l], acc[j]);
+                if (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);  // (all k's splits and reads at once would not fit the registers)
+            }
             if (sizeof(T) == 4 && __any(bad)) {  // an infinity: element by element (see Frag<float>)
                 for (int j = 0; j < 4; ++j)
                     for (int e = 0; e < 4; ++e) {
@@ -1003,14 +1021,15 @@ int launch_product(const Args& a, Shape sh, bool dma, unsigned blocks, hipStream
     }
 }
 
-// The strip kernel for contractions of up to 256 elements (fp32: 128) whose weights fit two workgroups' LDS: all of them, or, where
-// the contraction is so short (64) that reading P again for every q_tile columns costs little beside the output, any number.
+// The strip kernel for contractions of up to 256 elements whose weights fit the workgroups' LDS: all of them, or, where the contraction
+// is so short (64) that reading P again for every q_tile columns costs little beside the output, any number (256 -> 128 fp32, two
+// tiles: 387 us, the tile kernel 271).
 // Returns 0 where the tile kernel is to run.
 template <typename T>
 int strip_q_tile(int n_c, int n_q) {
     const int steps = ceil_div(n_c, 32), nc = steps <= 1 ? 1 : steps <= 2 ? 2 : steps <= 4 ? 4 : 8;
-    const int tile = kStripLds / (nc * 64 * Frag<T>::kPlanes) / 64 * 64;
-    if (steps > 8 || tile == 0 || (n_q > tile && nc > 2)) return 0;
+    const int tile = strip_lds<T>() / (nc * 64 * Frag<T>::kPlanes) / 64 * 64;
+    if (steps > 8 || (n_q > tile && nc > 2)) return 0;
     return ceil_div(n_q, 64) * 64 < tile ? ceil_div(n_q, 64) * 64 : tile;
 }
 
@@ -1034,8 +1053,7 @@ int launch_strip(const Args& a, int q_tile, hipStream_t s) {
     if (n_c <= 32) return launch_strip_n<T, PRODUCT, 1>(a, q_tile, (int)run, (unsigned)blocks, s);
     if (n_c <= 64) return launch_strip_n<T, PRODUCT, 2>(a, q_tile, (int)run, (unsigned)blocks, s);
     if (n_c <= 128) return launch_strip_n<T, PRODUCT, 4>(a, q_tile, (int)run, (unsigned)blocks, s);
-    if constexpr (sizeof(T) == 2) return launch_strip_n<T, PRODUCT, 8>(a, q_tile, (int)run, (unsigned)blocks, s);
-    return MCMC_EINVAL;  // strip_q_tile takes no fp32 contraction beyond 128
+    return launch_strip_n<T, PRODUCT, 8>(a, q_tile, (int)run, (unsigned)blocks, s);
 }
 
 // Parts of a long contraction (forward, dx) where the output has too few tiles to fill the chip: a step of one workgroup waits for
