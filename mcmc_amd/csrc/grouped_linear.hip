@@ -539,28 +539,51 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             if (g < FQ) fq[half][g] = q_frag(at, 0, g, half);
             if (g >= 1 && g - 1 < NT2) fp[g - 1] = p_frag(at, 0, g - 1, half);
         };
-        auto multiply = [&](auto with_bias, int i, int half) {
+        auto multiply = [&](int i, int half) {
             const V p = i < NT2 ? fp[i < NT2 ? i : 0] : tail[half][i < NT2 ? 0 : i - NT2];
 #pragma unroll
             for (int j = 0; j < FQ; ++j) acc[i][j] = F::mfma(fq[half][j], p, acc[i][j]);
-            if (decltype(with_bias)::value) accb[i] = add_elements(p, accb[i]);
         };
         if (steps > 0) {
             load_all(0, 0);
             load_all(1, 1);
             wait_loads<NL>();
             barrier_lds_only();
-#pragma unroll
-            for (int g = 0; g < FP; ++g) read_group(g, 0, 0);
         }
-        auto all_steps = [&](auto with_bias) {
+        if (PRODUCT == kGradWeight && sum_bias) {
+            // The waves that also sum dy's columns (those of the first output columns, one wave in 16 of a 4096 x 4096 dW) read each
+            // fragment where it is multiplied: the sums' registers beside two sets of fragments would be kept in memory, and every
+            // reload of one waits for all loads in flight.  They meet the others at the same barriers.
+            for (int s = 0; s < steps; ++s) {
+                const int now = s & 1;
+                if (s % (kSegment / BC) == 0) fetch_segment(s / (kSegment / BC) + 1);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int j = 0; j < FQ; ++j) fq[0][j] = q_frag(smem + now * kStage, 0, j, half);
+#pragma unroll
+                    for (int i = 0; i < FP; ++i) {
+                        const V p = p_frag(smem + now * kStage, 0, i, half);
+#pragma unroll
+                        for (int j = 0; j < FQ; ++j) acc[i][j] = F::mfma(fq[0][j], p, acc[i][j]);
+                        accb[i] = add_elements(p, accb[i]);
+                    }
+                }
+                wait_loads<0>();
+                barrier_lds_only();
+                load_all(s + 2, now);
+            }
+        } else {
+            if (steps > 0)
+#pragma unroll
+                for (int g = 0; g < FP; ++g) read_group(g, 0, 0);
             for (int s = 0; s < steps; ++s) {
                 const int now = s & 1;
                 if (s % (kSegment / BC) == 0) fetch_segment(s / (kSegment / BC) + 1);  // the segment before s's is no longer read
                 asm volatile("" : "+v"(at_p), "+v"(at_q));  // as now_lane: the fragments' offsets are made where they are used
 #pragma unroll
                 for (int g = 0; g < FP; ++g) {
-                    multiply(with_bias, g, 0);
+                    multiply(g, 0);
                     read_group(g, 1, now);
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -569,16 +592,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
                 look_up(s + 2);
 #pragma unroll
                 for (int g = 0; g < FP; ++g) {
-                    multiply(with_bias, g, 1);
+                    multiply(g, 1);
                     read_group(g, 0, now ^ 1);
 #pragma unroll
                     for (int n = g * NL / FP; n < (g + 1) * NL / FP; ++n) load(n, s + 2, now);  // past the last step: zeros, nobody reads them
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-        };
-        if (PRODUCT == kGradWeight && sum_bias) all_steps(std::integral_constant<bool, PRODUCT == kGradWeight>());
-        else all_steps(std::false_type());
+        }
         wait_loads<0>();  // no load may outlive its workgroup's LDS
     } else {
         // through registers: all of Q's fragments against one of P's after the other, which are read two ahead
