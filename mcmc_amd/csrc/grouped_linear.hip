@@ -377,10 +377,17 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     // ---- where this lane's pieces come from.  "rows": the chunk's address at step 0, kept.  "columns": row of the tile and first column,
     // made from the lane number where they are used: kept in registers for all pieces they would crowd out the accumulators
     // (`now_lane` is the lane number behind an empty asm statement, so that the compiler does not move the arithmetic out of the loop).
+    // A piece's row in the tile is a lane's part plus a wave's (col_row0), which share no bits that spread() looks at: the permutation is
+    // the exclusive or of theirs, and the wave's is scalar arithmetic.
     const T *src_p[kPCols ? 1 : NP], *src_q[kQCols ? 1 : NQ];
     int c_p = 0, c_q[kQCols ? 1 : NQ];  // "rows": first element of the chunk at step 0 (all of P's pieces of a lane have the same one)
     int now_lane = lane;
-    auto col_row = [&](int n, int np, int b) { return ((wave * np + n) * 64 + now_lane) / (b / 8); };
+    auto col_row0 = [&](int n, int np, int b) { return (wave * np + n) * (64 / (b / 8)); };
+    auto col_row = [&](int n, int np, int b) { return col_row0(n, np, b) + now_lane / (b / 8); };
+    auto column_of = [&](auto width, int n, int np) {
+        constexpr int B = decltype(width)::value;
+        return (8 * (now_lane % (B / 8)) ^ (spread<B>(now_lane / (B / 8)) >> 1)) ^ (spread<B>(col_row0(n, np, B)) >> 1);
+    };
     if constexpr (!kPCols) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
@@ -434,10 +441,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         unsigned to = lds_address(smem + stage * kStage);
         if (n < NP) {
             if constexpr (kPCols) {
-                const int c = col_row(n, NP, BP);
-                int col = p0 + 8 * ((((wave * NP + n) * 64 + now_lane) % (BP / 8)) ^ (spread<BP>(c) >> 4));
+                int col = p0 + column_of(std::integral_constant<int, BP>(), n, NP);
                 have = row_p[n] >= 0 ? (DMA ? 8 : n_p - col) : 0;
-                if (DMA && col >= n_p) col = 0;  // columns past the end: any, not stored
+                if (DMA) col = col < n_p - 8 ? col : n_p - 8;  // columns past the end: any, not stored
                 p = P + (int64_t)row_p[n] * a.ld_p + col;
             } else {
                 have = n_c - c0 - c_p;
@@ -448,11 +454,11 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             const int m = n - NP;
             if constexpr (kQCols) {
                 const int c = col_row(m, NQ, BQ);
-                int r, col = q0 + 8 * ((((wave * NQ + m) * 64 + now_lane) % (BQ / 8)) ^ (spread<BQ>(c) >> 4));
+                int r, col = q0 + column_of(std::integral_constant<int, BQ>(), m, NQ);
                 if constexpr (PRODUCT == kGradWeight) r = BP != BQ ? row_q[BP != BQ ? m : 0] : row_p[m];
                 else r = c0 + c < n_c ? c0 + c : -1;
                 have = r >= 0 ? (DMA ? 8 : n_q - col) : 0;
-                if (DMA && col >= n_q) col = 0;
+                if (DMA) col = col < n_q - 8 ? col : n_q - 8;
                 p = Q + (int64_t)r * a.ld_q + col;
             } else {
                 have = n_c - c0 - c_q[m];
