@@ -130,38 +130,21 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
 
 
 # ---- grouped_linear ---------------------------------------------------------------------------------------------------------
-def _workspace(eng: Engine, product: int, dt: int, R: int, G: int, K: int, N: int, dev) -> Optional[torch.Tensor]:
-    n = _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(product, dt, R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
+def _workspace_bytes(eng: Engine, product: int, dt: int, R: int, G: int, K: int, N: int) -> int:
+    return _lib.check(eng.lib.mcmc_grouped_linear_workspace_bytes(product, dt, R, G, K, N), "mcmc_grouped_linear_workspace_bytes")
+
+
+def _workspace(n: int, dev) -> Optional[torch.Tensor]:
     return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
 def _forward(eng: Engine, x, weight, bias, order, offsets):
-    (R, K), (G, N, _) = x.shape, weight.shape
-    dt, y = _DT[x.dtype], torch.empty((R, N), dtype=x.dtype, device=x.device)
-    ws = _workspace(eng, _lib.GROUPED_FORWARD, dt, R, G, K, N, x.device)
+    (R, K), (G, N, _), dev = x.shape, weight.shape, x.device
+    dt, y = _DT[x.dtype], torch.empty((R, N), dtype=x.dtype, device=dev)
+    ws = _workspace(_workspace_bytes(eng, _lib.GROUPED_FORWARD, dt, R, G, K, N), dev)
     _lib.check(eng.lib.mcmc_grouped_linear_forward(eng.ctx.handle, dt, x.data_ptr(), x.stride(0), R, _ptr(order), offsets.data_ptr(), G, K, N,
                                                    weight.data_ptr(), _ptr(bias), y.data_ptr(), _ptr(ws), _stream(eng)), "mcmc_grouped_linear_forward")
     return y
-
-
-def _grad_input(eng: Engine, dy, weight, order, offsets):
-    R, (G, N, K) = dy.shape[0], weight.shape
-    dt, dx = _DT[dy.dtype], torch.empty((R, K), dtype=dy.dtype, device=dy.device)
-    ws = _workspace(eng, _lib.GROUPED_GRAD_INPUT, dt, R, G, K, N, dy.device)
-    _lib.check(eng.lib.mcmc_grouped_linear_grad_input(eng.ctx.handle, dt, dy.data_ptr(), dy.stride(0), R, _ptr(order), offsets.data_ptr(), G, K, N,
-                                                      weight.data_ptr(), dx.data_ptr(), _ptr(ws), _stream(eng)), "mcmc_grouped_linear_grad_input")
-    return dx
-
-
-def _grad_weight(eng: Engine, dy, x, order, offsets, G: int, want_bias: bool):
-    (R, K), N, dt, dev = x.shape, dy.shape[1], _DT[x.dtype], x.device
-    ws = _workspace(eng, _lib.GROUPED_GRAD_WEIGHT, dt, R, G, K, N, dev)
-    dw = torch.empty((G, N, K), dtype=x.dtype, device=dev)
-    db = torch.empty((G, N), dtype=x.dtype, device=dev) if want_bias else None
-    _lib.check(eng.lib.mcmc_grouped_linear_grad_weight(eng.ctx.handle, dt, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), R, _ptr(order),
-                                                       offsets.data_ptr(), G, K, N, dw.data_ptr(), _ptr(db), _ptr(ws), _stream(eng)),
-               "mcmc_grouped_linear_grad_weight")
-    return dw, db
 
 
 class _GroupedLinear(torch.autograd.Function):
@@ -171,7 +154,10 @@ class _GroupedLinear(torch.autograd.Function):
             x, weight = _rows(x), weight.contiguous()
             y = _forward(eng, x, weight, None if bias is None else bias.contiguous(), order, offsets)
         need_x, need_w, need_b = ctx.needs_input_grad[1:4]
-        ctx.eng, ctx.shape = eng, weight.shape
+        (R, K), (G, N, _), dt = x.shape, weight.shape, _DT[x.dtype]
+        ctx.eng, ctx.sizes = eng, (dt, R, G, K, N, x.stride(0))
+        ctx.ws = (_workspace_bytes(eng, _lib.GROUPED_GRAD_INPUT, dt, R, G, K, N) if need_x else 0,
+                  _workspace_bytes(eng, _lib.GROUPED_GRAD_WEIGHT, dt, R, G, K, N) if need_w or need_b else 0)
         # what each gradient reads: dx the weights, dW the inputs
         ctx.save_for_backward(x if need_w or need_b else None, weight if need_x else None, order, offsets)
         return y
@@ -179,16 +165,28 @@ class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dy):
-        eng = ctx.eng
+        eng, (dt, R, G, K, N, ld_x), (ws_x, ws_w) = ctx.eng, ctx.sizes, ctx.ws
         x, weight, order, offsets = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[1:4]
+        _, need_x, need_w, need_b, _, _ = ctx.needs_input_grad
         dx = dw = db = None
         with _on(eng):
-            dy = _rows(dy)
+            lib, handle, stream, dtype, dev = eng.lib, eng.ctx.handle, _stream(eng), dy.dtype, dy.device
+            ld_dy = N
+            if not dy.is_contiguous():
+                dy = _rows(dy)
+                ld_dy = dy.stride(0)
+            dy_p, order_p, offsets_p = dy.data_ptr(), _ptr(order), offsets.data_ptr()
             if need_x:
-                dx = _grad_input(eng, dy, weight, order, offsets)
+                dx = torch.empty((R, K), dtype=dtype, device=dev)
+                ws = _workspace(ws_x, dev)
+                _lib.check(lib.mcmc_grouped_linear_grad_input(handle, dt, dy_p, ld_dy, R, order_p, offsets_p, G, K, N, weight.data_ptr(), dx.data_ptr(),
+                                                              _ptr(ws), stream), "mcmc_grouped_linear_grad_input")
             if need_w or need_b:
-                dw, db = _grad_weight(eng, dy, x, order, offsets, ctx.shape[0], need_b)
+                dw = torch.empty((G, N, K), dtype=dtype, device=dev)
+                db = torch.empty((G, N), dtype=dtype, device=dev) if need_b else None
+                ws = _workspace(ws_w, dev)
+                _lib.check(lib.mcmc_grouped_linear_grad_weight(handle, dt, dy_p, ld_dy, x.data_ptr(), ld_x, R, order_p, offsets_p, G, K, N, dw.data_ptr(),
+                                                               _ptr(db), _ptr(ws), stream), "mcmc_grouped_linear_grad_weight")
         return None, dx, dw if need_w else None, db, None, None
 
 
