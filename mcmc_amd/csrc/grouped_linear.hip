@@ -253,11 +253,15 @@ __device__ __forceinline__ Piece<T> load_eight(const T* p, int n) {
     return u;
 }
 template <typename T>
+__device__ __forceinline__ void keep_first(Piece<T>& u, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u.v[i] = i < n ? u.v[i] : (T)0.0f;
+}
+template <typename T>
 __device__ __forceinline__ Piece<T> load_through(const T* p, int n, bool inside) {
     if (__any(n > 0 && n < 8 && !inside)) return load_piece(p, n);
     Piece<T> u = load_eight(p, n);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) u.v[i] = i < n ? u.v[i] : (T)0.0f;
+    keep_first(u, n);
     return u;
 }
 
@@ -381,6 +385,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     // the exclusive or of theirs, and the wave's is scalar arithmetic.
     const T *src_p[kPCols ? 1 : NP], *src_q[kQCols ? 1 : NQ];
     int c_p = 0, c_q[kQCols ? 1 : NQ];  // "rows": first element of the chunk at step 0 (all of P's pieces of a lane have the same one)
+    unsigned has_next_p = 0, has_next_q = 0;  // "rows", !DMA: bit n: eight elements from anywhere in piece n's row are memory of the operand
     int now_lane = lane;
     auto col_row0 = [&](int n, int np, int b) { return (wave * np + n) * (64 / (b / 8)); };
     auto col_row = [&](int n, int np, int b) { return col_row0(n, np, b) + now_lane / (b / 8); };
@@ -394,6 +399,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             const int piece = (wave * NP + n) * 64 + lane, r = piece / (BC / 8), row = rows_lds[r] < 0 ? 0 : rows_lds[r];
             c_p = 8 * ((piece % (BC / 8)) ^ turn<BC, false>(r));
             src_p[n] = P + (int64_t)row * a.ld_p + c_p;  // rows past the end: any, not stored
+            if (row + 1 < rows && a.ld_p > 7) has_next_p |= 1u << n;
         }
     }
     if constexpr (!kQCols) {
@@ -402,6 +408,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             const int piece = (wave * NQ + n) * 64 + lane, r = piece / (BC / 8), row = q0 + r < n_q ? q0 + r : n_q - 1;
             c_q[n] = 8 * ((piece % (BC / 8)) ^ turn<BC, kPair>(r));
             src_q[n] = Q + (int64_t)row * a.ld_q + c_q[n];
+            if (row + 1 < n_q && a.ld_q > 7) has_next_q |= 1u << n;
         }
     }
     // dW: row numbers of the run's positions 1024 s .. 1024 s + 1023 -> LDS
@@ -421,6 +428,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     };
     Piece<T> hold_p[DMA ? 1 : NP], hold_q[DMA ? 1 : NQ];
     bool infinite = false;
+    int rest_p = 8, rest_q[kQCols ? 1 : NQ];  // "rows" in hold_*: elements before the contraction's end
     // dW: the rows of this lane's pieces, looked up before the pieces are asked for (both operands' pieces lie alike if BP == BQ)
     int row_p[kPCols ? NP : 1], row_q[kPCols && BP != BQ ? NQ : 1];
     auto look_up = [&](int step) {
@@ -433,23 +441,24 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
                 for (int n = 0; n < NQ; ++n) row_q[n] = row_of(step * BC + col_row(n, NQ, BQ));
         }
     };
-    // piece n (P's, then Q's) of a step; DMA: into LDS, otherwise into hold_*
-    auto load = [&](int n, int step, int stage) {
+    // Piece n (P's, then Q's) of a step: where it starts, how many of its elements exist, and whether eight may be read all the same (they
+    // end in a row that exists)
+    auto piece = [&](int n, int step, const T*& p, int& have, bool& inside) {
         const int c0 = step * BC;
-        const T* p;
-        int have;  // elements of the chunk that exist (DMA: all or none)
-        unsigned to = lds_address(smem + stage * kStage);
+        inside = true;
         if (n < NP) {
             if constexpr (kPCols) {
                 int col = p0 + column_of(std::integral_constant<int, BP>(), n, NP);
-                have = row_p[n] >= 0 ? (DMA ? 8 : n_p - col) : 0;
+                have = row_p[n] >= 0 ? n_p - col : 0;
                 if (DMA) col = col < n_p - 8 ? col : n_p - 8;  // columns past the end: any, not stored
+                else inside = row_p[n] + 1 < rows && col + 8 <= a.ld_p + n_p;
+                if (DMA) have = row_p[n] >= 0 ? 8 : 0;
                 p = P + (int64_t)row_p[n] * a.ld_p + col;
             } else {
                 have = n_c - c0 - c_p;
                 p = src_p[n] + c0;
+                if (!DMA) inside = has_next_p >> n & 1;
             }
-            to += (wave * NP + n) * 1024;
         } else {
             const int m = n - NP;
             if constexpr (kQCols) {
@@ -457,30 +466,73 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
                 int r, col = q0 + column_of(std::integral_constant<int, BQ>(), m, NQ);
                 if constexpr (PRODUCT == kGradWeight) r = BP != BQ ? row_q[BP != BQ ? m : 0] : row_p[m];
                 else r = c0 + c < n_c ? c0 + c : -1;
-                have = r >= 0 ? (DMA ? 8 : n_q - col) : 0;
+                have = r >= 0 ? n_q - col : 0;
                 if (DMA) col = col < n_q - 8 ? col : n_q - 8;
+                else inside = r + 1 < (PRODUCT == kGradWeight ? rows : n_c) && col + 8 <= a.ld_q + n_q;
+                if (DMA) have = r >= 0 ? 8 : 0;
                 p = Q + (int64_t)r * a.ld_q + col;
             } else {
                 have = n_c - c0 - c_q[m];
                 p = src_q[m] + c0;
+                if (!DMA) inside = has_next_q >> m & 1;
             }
-            to += kPBytes * F::kPlanes + (wave * NQ + m) * 1024;
         }
-        if (DMA) glds16(have > 0 ? p : zeros, __builtin_amdgcn_readfirstlane(to));
-        else if (n < NP) hold_p[DMA || n >= NP ? 0 : n] = load_piece(p, have);
-        else hold_q[DMA || n < NP ? 0 : n - NP] = load_piece(p, have);
     };
-    auto load_all = [&](int step, int stage) {
+    auto load = [&](int n, int step, int stage) {  // DMA: into LDS
+        const T* p;
+        int have;
+        bool inside;
+        piece(n, step, p, have, inside);
+        const unsigned to = lds_address(smem + stage * kStage) + (n < NP ? (wave * NP + n) * 1024 : kPBytes + (wave * NQ + n - NP) * 1024);
+        glds16(have > 0 ? p : zeros, __builtin_amdgcn_readfirstlane(to));
+    };
+    auto load_all = [&](int step, int stage) {  // !DMA: into hold_*, no branch between the loads
         look_up(step);
+        if constexpr (DMA) {
 #pragma unroll
-        for (int n = 0; n < NP + NQ; ++n) load(n, step, stage);
+            for (int n = 0; n < NP + NQ; ++n) load(n, step, stage);
+        } else {
+            const T* p[NP + NQ];
+            int have[NP + NQ];
+            bool beyond = false;  // a piece that is not whole and has no row after its own
+#pragma unroll
+            for (int n = 0; n < NP + NQ; ++n) {
+                bool inside;
+                piece(n, step, p[n], have[n], inside);
+                beyond |= have[n] > 0 && have[n] < 8 && !inside;
+            }
+            const bool slow = __any(beyond);
+            if (!slow) {
+#pragma unroll
+                for (int n = 0; n < NP; ++n) hold_p[n] = load_eight(p[n], have[n]);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) hold_q[n] = load_eight(p[NP + n], have[NP + n]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < NP; ++n) hold_p[n] = load_piece(p[n], have[n]);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) hold_q[n] = load_piece(p[NP + n], have[NP + n]);
+            }
+            // what was read past an operand's contraction is dropped when it is stored (past its output columns, it does not matter)
+            if constexpr (!kPCols) rest_p = have[0];
+            if constexpr (!kQCols)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) rest_q[n] = have[NP + n];
+        }
     };
+    const bool ragged = n_c % 8 != 0;
     auto store = [&](int stage) {
         char* s = smem + stage * kStage;
 #pragma unroll
-        for (int n = 0; n < NP; ++n) store_piece(s + ((wave * NP + n) * 64 + lane) * 16, kPBytes, hold_p[DMA ? 0 : n], infinite);
+        for (int n = 0; n < NP; ++n) {
+            if (!DMA && !kPCols && ragged) keep_first(hold_p[DMA ? 0 : n], rest_p);
+            store_piece(s + ((wave * NP + n) * 64 + lane) * 16, kPBytes, hold_p[DMA ? 0 : n], infinite);
+        }
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) store_piece(s + F::kPlanes * kPBytes + ((wave * NQ + n) * 64 + lane) * 16, kQBytes, hold_q[DMA ? 0 : n], infinite);
+        for (int n = 0; n < NQ; ++n) {
+            if (!DMA && !kQCols && ragged) keep_first(hold_q[DMA ? 0 : n], rest_q[kQCols ? 0 : n]);
+            store_piece(s + F::kPlanes * kPBytes + ((wave * NQ + n) * 64 + lane) * 16, kQBytes, hold_q[DMA ? 0 : n], infinite);
+        }
     };
 
     // ---- fragments
@@ -870,11 +922,35 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
 }
 
 // ---- dW where one side is a handful of columns (the output layer, the first layer) ------------------------------------------------
-// dW[t][c] = sum_r thin[r][t] wide[r][c], at most 16 columns t: bound by reading the wide rows once.  On the fp32 matrix
-// instructions (16 x 16 outputs, 4 rows each), whose operands need no turning: lane (fr, kg) holds thin[row kg][fr] and, for instruction
-// j, wide[row kg][8 fr + j] - it loads its 8 columns of a row in one access and 16 lanes load a row's 128 side by side.  Exact for
-// 16-bit operands, plain fp32 sums for fp32.  Four waves take turns at 64 rows of a run and meet in LDS in their order.
+// dW[t][c] = sum_r thin[r][t] wide[r][c], at most 16 columns t: bound by reading the wide rows once.  On matrix instructions of
+// 16 x 16 outputs whose lane (fr, kg) holds kRows rows of one column: it loads its 8 columns 8 fr .. of rows kRows kg + r of both in
+// whole accesses (16 lanes read a row's 128 columns side by side), and instruction j takes column 8 fr + j of them, so nothing is
+// turned through LDS.  16-bit: 16 rows an instruction, four rows' halves brought together; fp32: the fp32 instruction, 4 rows.
+// Four waves take turns at 64 rows of a run and meet in LDS in their order.
 // THIN_OUT: thin = dy (n_out columns), db is its column sum; otherwise thin = x (n_in <= 15), and db comes from a column of ones.
+template <typename T>
+struct ThinFrag;
+template <>
+struct ThinFrag<float> {
+    typedef float V;
+    static constexpr int kRows = 1;
+    static __device__ __forceinline__ void put(V& v, int, float x) { v = x; }
+    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 d) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, d, 0, 0, 0); }
+};
+template <>
+struct ThinFrag<__bf16> {
+    typedef s16x4 V;
+    static constexpr int kRows = 4;
+    static __device__ __forceinline__ void put(V& v, int r, __bf16 x) { v[r] = __builtin_bit_cast(short, x); }
+    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 d) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, d, 0, 0, 0); }
+};
+template <>
+struct ThinFrag<_Float16> {
+    typedef _Float16 V __attribute__((ext_vector_type(4)));
+    static constexpr int kRows = 4;
+    static __device__ __forceinline__ void put(V& v, int r, _Float16 x) { v[r] = x; }
+    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 d) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, d, 0, 0, 0); }
+};
 constexpr int kThinMost = 16;
 constexpr int kThinCols = 128;
 
@@ -899,36 +975,54 @@ __global__ __launch_bounds__(256) void grouped_thin_kernel(Args a) {
     const int c = w0 + 8 * fr;
     f32x4 acc[8] = {};
     float sum_b = 0.0f;
+    typedef ThinFrag<T> F;
+    constexpr int KR = F::kRows, kSteps = 64 / (4 * KR), kAtOnce = KR == 1 ? 4 : 2;  // loads in flight: 4 (fp32: of 32 bytes), 8 rows a lane
+    int mine = tl.first + 64 * wave + lane < tl.last ? row_at(a, tl.first + 64 * wave + lane) : -1;
     for (int first = tl.first + 64 * wave; first < tl.last; first += 256) {
-        const int mine = first + lane < tl.last ? row_at(a, first + lane) : -1;
+        const int next = first + 256 + lane < tl.last ? row_at(a, first + 256 + lane) : -1;
 #pragma unroll 1
-        for (int s0 = 0; s0 < 16; s0 += 4) {
-            Piece<T> w[4];
-            T th[4];
-            int row[4];
+        for (int s0 = 0; s0 < kSteps; s0 += kAtOnce) {
+            Piece<T> w[kAtOnce][KR];
+            T th[kAtOnce][KR];
+            int row[kAtOnce][KR];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                row[s] = __shfl(mine, 4 * (s0 + s) + kg);
-                th[s] = *(row[s] >= 0 && fr < n_t ? thin + (int64_t)row[s] * ld_t + fr : reinterpret_cast<const T*>(kZeros));
-            }
+            for (int s = 0; s < kAtOnce; ++s)
+#pragma unroll
+                for (int r = 0; r < KR; ++r) {
+                    row[s][r] = __shfl(mine, 4 * KR * (s0 + s) + KR * kg + r);
+                    th[s][r] = *(row[s][r] >= 0 && fr < n_t ? thin + (int64_t)row[s][r] * ld_t + fr : reinterpret_cast<const T*>(kZeros));
+                }
             if (n_w % 8 == 0) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) w[s] = load_eight(wide + (int64_t)row[s] * ld_w + c, row[s] < 0 ? 0 : n_w - c);
+                for (int s = 0; s < kAtOnce; ++s)
+#pragma unroll
+                    for (int r = 0; r < KR; ++r) w[s][r] = load_eight(wide + (int64_t)row[s][r] * ld_w + c, row[s][r] < 0 ? 0 : n_w - c);
             } else {
 #pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    w[s] = load_through(wide + (int64_t)row[s] * ld_w + c, row[s] < 0 ? 0 : n_w - c, row[s] + 1 < rows && c + 8 <= ld_w + n_w);
+                for (int s = 0; s < kAtOnce; ++s)
+#pragma unroll
+                    for (int r = 0; r < KR; ++r)
+                        w[s][r] = load_through(wide + (int64_t)row[s][r] * ld_w + c, row[s][r] < 0 ? 0 : n_w - c, row[s][r] + 1 < rows && c + 8 <= ld_w + n_w);
             }
-            if (!THIN_OUT && fr == n_t)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) th[s] = row[s] >= 0 ? (T)1.0f : (T)0.0f;
+            for (int s = 0; s < kAtOnce; ++s) {
+                typename F::V tv;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                if (THIN_OUT) sum_b += (float)th[s];
+                for (int r = 0; r < KR; ++r) {
+                    if (!THIN_OUT && fr == n_t) th[s][r] = row[s][r] >= 0 ? (T)1.0f : (T)0.0f;
+                    if (THIN_OUT) sum_b += (float)th[s][r];
+                    F::put(tv, r, th[s][r]);
+                }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)th[s], (float)w[s].v[j], acc[j], 0, 0, 0);
+                for (int j = 0; j < 8; ++j) {
+                    typename F::V wv;
+#pragma unroll
+                    for (int r = 0; r < KR; ++r) F::put(wv, r, w[s][r].v[j]);
+                    acc[j] = F::mfma(tv, wv, acc[j]);
+                }
             }
         }
+        mine = next;
     }
     // lane: thin columns 4 kg + i, wide columns 8 fr + j
 #pragma unroll
