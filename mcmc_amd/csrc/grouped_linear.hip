@@ -223,20 +223,24 @@ __device__ __forceinline__ Piece<T> load_piece(const T* p, int n) {
     }
     return u;
 }
+// largest: of the fp32 elements as rounded to bf16, infinite if one of them is (a NaN is passed over)
 template <typename T>
-__device__ __forceinline__ void store_piece(char* at, int plane_bytes, const Piece<T>& u, bool& infinite) {
+__device__ __forceinline__ void store_piece(char* at, int plane_bytes, const Piece<T>& u, float& largest) {
     if constexpr (sizeof(T) == 2) {
         __builtin_memcpy(__builtin_assume_aligned(at, 16), u.v, 16);
     } else {
         bf16x8 h, m, l;
+        float hi[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             h[i] = (__bf16)u.v[i];
-            const float hi = (float)h[i], rest = u.v[i] - hi;
-            infinite |= __builtin_isinf(hi);
+            hi[i] = (float)h[i];
+            const float rest = u.v[i] - hi[i];
             m[i] = (__bf16)rest;
             l[i] = (__bf16)(rest - (float)m[i]);
         }
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(largest) : "v"(hi[i]), "v"(hi[i + 1]));
         *reinterpret_cast<bf16x8*>(at) = h;
         *reinterpret_cast<bf16x8*>(at + plane_bytes) = m;
         *reinterpret_cast<bf16x8*>(at + 2 * plane_bytes) = l;
@@ -436,7 +440,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         return (unsigned)r < (unsigned)rows ? r : -1;
     };
     Piece<T> hold_p[DMA ? 1 : NP], hold_q[DMA ? 1 : NQ];
-    bool infinite = false;
+    float largest = 0.0f;
     int rest_p = 8, rest_q[kQCols ? 1 : NQ];  // "rows" in hold_*: elements before the contraction's end
     // dW: the rows of this lane's pieces, looked up before the pieces are asked for (both operands' pieces lie alike if BP == BQ)
     int row_p[kPCols ? NP : 1], row_q[kPCols && BP != BQ ? NQ : 1];
@@ -535,12 +539,12 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             if (!DMA && !kPCols && ragged) keep_first(hold_p[DMA ? 0 : n], rest_p);
-            store_piece(s + ((wave * NP + n) * 64 + lane) * 16, kPBytes, hold_p[DMA ? 0 : n], infinite);
+            store_piece(s + ((wave * NP + n) * 64 + lane) * 16, kPBytes, hold_p[DMA ? 0 : n], largest);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             if (!DMA && !kQCols && ragged) keep_first(hold_q[DMA ? 0 : n], rest_q[kQCols ? 0 : n]);
-            store_piece(s + F::kPlanes * kPBytes + ((wave * NQ + n) * 64 + lane) * 16, kQBytes, hold_q[DMA ? 0 : n], infinite);
+            store_piece(s + F::kPlanes * kPBytes + ((wave * NQ + n) * 64 + lane) * 16, kQBytes, hold_q[DMA ? 0 : n], largest);
         }
     };
 
@@ -720,7 +724,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
     }
     if constexpr (kWide) {
         // an infinity among the operands: the sums again, element by element from memory (rare, and as slow as that sounds)
-        if (__syncthreads_or(infinite)) {
+        if (__syncthreads_or(__builtin_isinf(largest))) {
             for (int i = 0; i < FP; ++i) {
                 const int p = pw + 16 * i + fr, row = kPCols ? 0 : rows_lds[p];
                 sumb[i] = accb[i] = 0.0f;
@@ -823,7 +827,7 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
     const T* const P = static_cast<const T*>(a.p);
     const T* const W = static_cast<const T*>(a.q) + (none ? 0 : (int64_t)tl.g * a.n_in * a.n_out);
     float* const bias = reinterpret_cast<float*>(smem + PL * plane_bytes);
-    bool infinite = false;
+    float largest = 0.0f;
 
     // ---- weights and bias -> LDS.  Piece (column, eight contraction elements): consecutive lanes take consecutive columns in dx (W's
     // rows are read along), consecutive chunks of a column in the forward pass
@@ -840,11 +844,11 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
         }
         const int in = col & 63, j = sizeof(T) == 4 ? in >> 4 : 2 * (in >> 5) + ((in >> 2) & 1);
         const int m = sizeof(T) == 4 ? in & 15 : 4 * ((in >> 3) & 3) + (in & 3);
-        store_piece(smem + ((((col >> 6) * 4 + j) * NC + (ch >> 2)) * 64 + (ch & 3) * 16 + m) * 16, plane_bytes, u, infinite);
+        store_piece(smem + ((((col >> 6) * 4 + j) * NC + (ch >> 2)) * 64 + (ch & 3) * 16 + m) * 16, plane_bytes, u, largest);
     }
     for (int i = t; i < blocks * 64; i += NT)
         bias[i] = PRODUCT == kForward && a.bias && !none && q0 + i < n_q ? (float)static_cast<const T*>(a.bias)[(int64_t)tl.g * a.n_out + q0 + i] : 0.0f;
-    infinite = __syncthreads_or(infinite);
+    const bool infinite = __syncthreads_or(__builtin_isinf(largest));
 
     auto row_of = [&](int first) { return first + fr < tl.last ? row_at(a, first + fr) : -1; };
     auto load_one = [&](int row, int k) {
@@ -873,7 +877,7 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
         row = row_next;
         T* const out = static_cast<T*>(a.out) + (int64_t)(out_row < 0 ? 0 : out_row) * n_q + q0;
         V p[sizeof(T) == 4 ? 1 : NC];
-        bool bad = infinite;
+        largest = 0.0f;
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int k = 0; k < NC; ++k) __builtin_memcpy(&p[k], u[k].v, 16);
@@ -894,7 +898,7 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
 #pragma unroll
                     for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(u[k].v[e]));
                     char planes[PL * 16];
-                    store_piece(planes, 16, u[k], bad);
+                    store_piece(planes, 16, u[k], largest);
                     if (b + 1 == blocks && more) {
                         int next = row;
                         asm volatile("" : "+v"(next));
@@ -911,7 +915,7 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
                         for (int j = 0; j < 4; ++j) acc[j] = F::mfma(*reinterpret_cast<const V*>(w + m * plane_bytes + (j * NC + k) * 1024), q[l], acc[j]);
                 if (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);  // (all k's splits and reads at once would not fit the registers)
             }
-            if (sizeof(T) == 4 && __any(bad)) {  // an infinity: element by element (see Frag<float>)
+            if (sizeof(T) == 4 && (infinite || __any(__builtin_isinf(largest)))) {  // an infinity: element by element (see Frag<float>)
                 for (int j = 0; j < 4; ++j)
                     for (int e = 0; e < 4; ++e) {
                         const int q = q0 + column(b, j) + e;
