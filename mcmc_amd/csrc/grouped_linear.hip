@@ -1179,14 +1179,21 @@ int launch_strip_n(const Args& a, int q_tile, int run, unsigned blocks, hipStrea
 template <typename T, int PRODUCT>
 int launch_strip(const Args& a, int q_tile, hipStream_t s) {
     const int n_q = PRODUCT == kForward ? a.n_out : a.n_in, n_c = PRODUCT == kForward ? a.n_in : a.n_out;
-    // rows per workgroup: about two workgroups a CU and round, whole turns of its waves, weights loaded once for many rows
-    int64_t run = a.rows / 1024 / (16 * kStripWaves) * (16 * kStripWaves);
-    run = run < 16 * kStripWaves ? 16 * kStripWaves : run > 4096 ? 4096 : run;
+    // Rows per workgroup, whole turns of its waves: eight times the bytes of its weights in LDS and 4 KB, for what it costs to start (a workgroup
+    // with fewer rows spends its time there, one with more leaves a long tail: 1,048,576 rows 11 -> 256 bf16: 1,024 rows 205 us, 256 rows 161; 256 -> 11
+    // fp32: 200 and 264), but no fewer workgroups than 1,024 as long as each has a turn.
+    const int nc = n_c <= 32 ? 1 : n_c <= 64 ? 2 : n_c <= 128 ? 4 : 8;
+    const int64_t weights = (int64_t)nc * 64 * Frag<T>::kPlanes * q_tile, row = (int64_t)sizeof(T) * (n_c + (n_q < q_tile ? n_q : q_tile));
+    constexpr int kTurn = 16 * kStripWaves;
+    int64_t run = 8 * (weights + 4096) / row;
+    run = a.rows / 1024 < run ? a.rows / 1024 : run;
+    run = run / kTurn * kTurn;
+    run = run < kTurn ? kTurn : run;
     const int64_t blocks = (a.rows / run + (a.G + 1 < a.rows ? a.G + 1 : a.rows)) * ceil_div(n_q, q_tile);
     if (int rc = check_grid(blocks)) return rc;
-    if (n_c <= 32) return launch_strip_n<T, PRODUCT, 1>(a, q_tile, (int)run, (unsigned)blocks, s);
-    if (n_c <= 64) return launch_strip_n<T, PRODUCT, 2>(a, q_tile, (int)run, (unsigned)blocks, s);
-    if (n_c <= 128) return launch_strip_n<T, PRODUCT, 4>(a, q_tile, (int)run, (unsigned)blocks, s);
+    if (nc == 1) return launch_strip_n<T, PRODUCT, 1>(a, q_tile, (int)run, (unsigned)blocks, s);
+    if (nc == 2) return launch_strip_n<T, PRODUCT, 2>(a, q_tile, (int)run, (unsigned)blocks, s);
+    if (nc == 4) return launch_strip_n<T, PRODUCT, 4>(a, q_tile, (int)run, (unsigned)blocks, s);
     return launch_strip_n<T, PRODUCT, 8>(a, q_tile, (int)run, (unsigned)blocks, s);
 }
 
