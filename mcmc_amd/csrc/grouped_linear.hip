@@ -1118,7 +1118,9 @@ Shape shape_of(int product, bool dma, int64_t rows, int G, int n_in, int n_out) 
 int chunk_rows_of(int64_t rows, int G, int n_in, int n_out) {
     const int64_t tiles = (int64_t)ceil_div(n_out, 128) * ceil_div(n_in, 128);
     if (tiles * G >= 512 || rows <= 512) return 0;
-    int64_t per = ceil_div(rows * tiles, tiles <= 4 ? 1024 : 512);  // (the larger dW is, the more its partial sums cost)
+    // as many as run at once, two workgroups a CU, counting the short chunk that ends each group: no tail, and no more partial sums
+    // than that takes (524,288 rows, 8 groups, 256 x 128 fp32: 289 us, twice as many chunks 333)
+    int64_t per = ceil_div(rows * tiles, tiles * G < 256 ? 512 - tiles * G : 256);
     per = (per + 255) / 256 * 256;
     return per >= rows ? 0 : (int)per;
 }
