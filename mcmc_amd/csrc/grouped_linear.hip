@@ -186,7 +186,13 @@ constexpr int kThreads = 256;
 //   on the global side, a wave-instruction fills 1 KiB of LDS in order), 16 zero bytes stand in for what lies past the
 //   contraction's end.  Otherwise they pass through registers, element by element where a chunk crosses the end of a row.
 // fp32, one LDS stage (three planes are 48 KB at 128 x 128 x 32: two workgroups a CU, one multiplies while the other stages): the
-// loads of step t+1 are in registers while step t is multiplied, and are split on their way into LDS.
+// loads of step t+1 are in registers while step t is multiplied, and are split on their way into LDS.  (Two stages of 256 x 128, one
+// workgroup a CU, the splitting between the products: the same at 2048 x 2048, 15 % slower at 256 x 128.)
+// Measured, 16-bit, 32,768 rows, 4096 x 4096: one group 835 / 902 / 1,020 us (forward, dx, dW: 1,317 / 1,219 / 1,078 TFLOP/s), where the
+// clock falls to what the power allows; eight groups of random sizes 1,001 / 1,030 / 1,065 (136 row tiles for 128: nine rounds of
+// workgroups for eight).  8,192 rows, 8 groups, 2048 x 2048: 97 / 105 / 82 us, 707 / 656 / 834 TFLOP/s; rows that are not whole 16-byte
+// pieces (2047 x 2045) 214 / 180 / 160.  fp32 there: 472 / 469 / 422 us, 146 / 147 / 163 TFLOP/s (the fp32 matrix instructions' dense
+// product reaches 153 on this card).
 __device__ const uint4 kZeros[2] = {};
 constexpr int kSegment = 1024;  // dW: row numbers in LDS, two segments, the next one loaded while one is used
 
@@ -804,6 +810,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 // A lane's results are four columns (m = 4 kg .. 4 kg + 3) of each of a 64-column block's four fragments.  fp32: fragment j holds columns
 // 16 j + m.  16-bit: fragments 2 h and 2 h + 1 hold columns 32 h + 8 (m >> 2) + 4 (j & 1) + (m & 3), so that two of them are eight
 // consecutive columns.  Either way a lane stores 16 bytes at a time and the four lanes of a row 64 consecutive bytes.
+// Measured, bf16, 8 groups, forward / dx (the tile kernel): 3,650,000 rows 256 -> 128 611 / 643 us (668 / 787), 4.6 / 4.4 TB/s; 1,048,576
+// rows 128 -> 64 97 / 103 (130 / 121), 64 -> 1 41 / 36 (94 / 77), 11 -> 256 161 / 152 (200 / 201).
 constexpr int kStripWaves = 8;
 // LDS for a workgroup's weights: two workgroups a CU; fp32, whose registers allow one, most of it
 template <typename T>
@@ -939,7 +947,8 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
 // 16 x 16 outputs whose lane (fr, kg) holds kRows rows of one column: it loads its 8 columns 8 fr .. of rows kRows kg + r of both in
 // whole accesses (16 lanes read a row's 128 columns side by side), and instruction j takes column 8 fr + j of them, so nothing is
 // turned through LDS.  16-bit: 16 rows an instruction, four rows' halves brought together; fp32: the fp32 instruction, 4 rows.
-// Four waves take turns at 64 rows of a run and meet in LDS in their order.
+// Four waves take turns at 64 rows of a run and meet in LDS in their order.  1,048,576 rows, 8 groups, bf16, with the chunks' sum
+// (the tile kernel): 64 -> 1 49 us (189), 2.8 TB/s; 64 -> 16 51 (64); 11 -> 256 128 (206), 4.4 TB/s.
 // THIN_OUT: thin = dy (n_out columns), db is its column sum; otherwise thin = x (n_in <= 15), and db comes from a column of ones.
 template <typename T>
 struct ThinFrag;
@@ -1105,6 +1114,10 @@ __global__ __launch_bounds__(kThreads) void grouped_join_kernel(const float* __r
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// 256 x 256 outputs a workgroup read each operand half as often as 128 x 128 (32,768 rows, 8 groups, 4096 x 4096: 1,043 / 1,076 / 1,114 us
+// against 1,289 / 1,380 / 1,577), but there is one workgroup a CU, and it is not worth its start where few tiles or few rows fill it:
+// less than a tile a CU (dW of 1024 x 1024, 8 groups: 74 us against 54; of 512 x 512 in chunks: 160 against 117), groups below a tile
+// (125 rows each, 1024 x 1024: 27 against 18 us).  Between (1024 x 1024, 2,000 rows a group) the two are within 10 %.
 struct Shape {
     int bp, bq;
 };
@@ -1114,7 +1127,8 @@ Shape shape_of(int product, bool dma, int64_t rows, int G, int n_in, int n_out) 
     return dma && n_p >= 192 && n_q >= 192 && tiles >= 256 ? Shape{256, 256} : Shape{128, 128};
 }
 
-// rows per partial sum of dW: 0 (no split) when the output tiles alone fill the chip
+// rows per partial sum of dW: 0 (no split) when the output tiles alone fill the chip (65,536 rows, 8 groups, 512 x 512: 161 us whole, 88
+// in chunks; 1,048,576 rows 128 -> 64: 2,687 and 88)
 int chunk_rows_of(int64_t rows, int G, int n_in, int n_out) {
     const int64_t tiles = (int64_t)ceil_div(n_out, 128) * ceil_div(n_in, 128);
     if (tiles * G >= 512 || rows <= 512) return 0;
@@ -1159,7 +1173,7 @@ int launch_product(const Args& a, Shape sh, bool dma, unsigned blocks, hipStream
 
 // The strip kernel for contractions of up to 256 elements whose weights fit the workgroups' LDS: all of them, or, where the contraction
 // is so short (64) that reading P again for every q_tile columns costs little beside the output, any number (256 -> 128 fp32, two
-// tiles: 387 us, the tile kernel 271).
+// tiles: 330 us, the tile kernel 261).
 // Returns 0 where the tile kernel is to run.
 template <typename T>
 int strip_q_tile(int n_c, int n_q) {
@@ -1254,7 +1268,8 @@ int launch(int product, Args a, hipStream_t s) {
         return rc;
     }
     if (!a.chunk_rows) return MCMC_OK;
-    // few chunks a group: a thread sums them all; many: eight threads share them
+    // few chunks a group: a thread sums them all; many: eight threads share them (1,048,576 rows in one group, 504 chunks, 64 -> 1: 49 us
+    // in all, 65 with one thread; up to 64 chunks the same)
     const int slices = a.chunks / a.G > 16 ? 8 : 1;
     const int64_t sums = ((int64_t)a.n_out * a.n_in + (a.dbias ? a.n_out : 0) + kThreads / slices - 1) / (kThreads / slices) * a.G;
     if (int rc = check_grid(sums)) return rc;
