@@ -11,7 +11,8 @@ product runs over the ragged groups in one launch:
 
 All arithmetic is in libmcmc_hip.so (``mcmc_group_rows``, ``mcmc_grouped_linear_*``, ``mcmc_dropout_*``); gradients are ordinary
 autograd.  There is no CPU path.  Every call runs on the current stream of its tensors' device and allocates what it needs from
-torch, nothing is kept from one call for the next, so calls may be captured into HIP graphs.
+torch, nothing is kept from one call for the next, so calls may be captured into HIP graphs (after a first call outside the
+capture, which loads the kernels; a backward pass, as torch has it, only while no eager graph of the same leaves is alive).
 """
 from __future__ import annotations
 
@@ -267,7 +268,7 @@ def philox_dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], *,
 
     The last dimension of x holds a row's elements, the others count rows (row-major).  Column c of row r is element
     ``elem_begin + c`` of row ``row_begin + r`` of ``pair``: a batch cut into pieces draws the same masks as the whole with
-    ``row_begin`` set, and elem_begin 0 / 256 / 384 with a pair's global id gives the masks of ``mcmc_train_forward``'s three
+    ``row_begin`` set, and elem_begin (a multiple of 16) 0 / 256 / 384 with a pair's global id gives the masks of ``mcmc_train_forward``'s three
     hidden layers.  A dropped element is 0 whatever x holds there.
 
     activation: None or "elu" (alpha 1), applied before the dropout.  p in [0, 1); the keep probability is (1 - p) rounded down
