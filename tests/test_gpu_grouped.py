@@ -596,3 +596,45 @@ def test_long_contractions_on_few_tiles(R, G, K, N, dtype):
         for n in ref:
             check(got[n], ref[n], mag[n] * U, n)
         assert not got["y"][ids < 0].any() and not got["dx"][ids < 0].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", [(16_700, 3, 1032, 1024), (20_003, 5, 264, 2056), (4200, 16, 1032, 1000), (3000, 1, 4096, 4096)])
+def test_enough_tiles_for_every_cu(R, G, K, N, dtype):
+    """What fills the chip with 256 x 256 outputs a workgroup: y and dx of the first, y of the second, dW of the others (the last one's single group on all XCDs)."""
+    for ordered in (False, True):
+        x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, 23, ordered, 0.03, (1,) if G > 2 else ())
+        got = run_linear(x, w, b, dy, groups)
+        ref, mag = linear_reference(x, w, b, dy, ids)
+        for n in ref:
+            check(got[n], ref[n], mag[n] * U, f"{n} ordered={ordered}")
+        again = run_linear(x, w, b, dy, groups)
+        assert all(torch.equal(got[n], again[n]) for n in got), "the same bits every time"
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", [(600_001, 3, 64, 16), (300_000, 4, 11, 256), (400_003, 2, 255, 31)])
+def test_many_rows_past_weights_in_lds(R, G, K, N, dtype):
+    """Runs of several turns of a workgroup's waves, the last one of each group short."""
+    x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, 29, False, 0.02)
+    got = run_linear(x, w, b, dy, groups)
+    ref, mag = linear_reference(x, w, b, dy, ids)
+    for n in ref:
+        check(got[n], ref[n], mag[n] * U, n)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", [(1, 1, 1, 1), (365, 5, 11, 256), (100_000, 3, 64, 1), (200_001, 7, 11, 40), (150_000, 2, 128, 64), (70_000, 5, 300, 130),
+                                        (16_700, 3, 1032, 1024), (4200, 16, 1032, 1000), (3000, 1, 4096, 4096), (9, 2, 4096, 512), (5000, 100, 65, 33)])
+def test_small_integers_are_exact(R, G, K, N, dtype):
+    """Operands of -1, 0 and 1: every sum is an integer below 2^24, exact in 32 bits in any order, so that a row too many or too few shows
+    whatever the length; the result is its one rounding to the type."""
+    g = gen(31)
+    ids = torch.randint(0, G, (R,), generator=g, device=DEV)
+    ids[torch.rand(R, generator=g, device=DEV) < 0.5] = G // 2  # one group has half of the rows
+    ids[torch.rand(R, generator=g, device=DEV) < 0.05] = -1
+    x, w, b, dy = (torch.randint(-1, 2, s, generator=g, device=DEV).to(dtype) for s in ((R, K), (G, N, K), (G, N), (R, N)))
+    got = run_linear(x, w, b, dy, group_rows(ids, G))
+    ref, _ = linear_reference(x, w, b, dy, ids)
+    for n in ref:
+        assert torch.equal(got[n], ref[n].to(dtype)), n
