@@ -83,8 +83,9 @@ struct Frag<_Float16> {
 // fp32 on the bf16 pipe: the fp32 matrix instructions run at 1/16 of its rate.  x = h + m + l with h = x rounded to bf16's 8 bits, m =
 // the rest rounded likewise, l = what is left (at most 8 bits: exact, down to 2^-126); of the nine products the six down to h l +
 // m m + l h are summed in fp32, the small ones first, so that a short sum is rounded once.  Left out: m l + l m + l l, below
-// 2^-26 |x y|, a quarter of an fp32 rounding.  What rounds to an infinity has no such split (inf - inf): a workgroup that meets one
-// does its tile over, element by element.
+// 2^-26 |x y|, a quarter of an fp32 rounding.  Near the top of the range the six are not the product: an operand that rounds to an
+// infinity has no such split (inf - inf), of a product that overflows, or nearly does, some terms are infinite and of either sign.  All of
+// these end in a sum that is not finite, and infinities and NaN stay: such a sum is done over, one product after the other (plain_sums).
 template <>
 struct Frag<float> {
     typedef __bf16 E;
@@ -229,24 +230,19 @@ __device__ __forceinline__ Piece<T> load_piece(const T* p, int n) {
     }
     return u;
 }
-// largest: of the fp32 elements as rounded to bf16, infinite if one of them is (a NaN is passed over)
 template <typename T>
-__device__ __forceinline__ void store_piece(char* at, int plane_bytes, const Piece<T>& u, float& largest) {
+__device__ __forceinline__ void store_piece(char* at, int plane_bytes, const Piece<T>& u) {
     if constexpr (sizeof(T) == 2) {
         __builtin_memcpy(__builtin_assume_aligned(at, 16), u.v, 16);
     } else {
         bf16x8 h, m, l;
-        float hi[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             h[i] = (__bf16)u.v[i];
-            hi[i] = (float)h[i];
-            const float rest = u.v[i] - hi[i];
+            const float rest = u.v[i] - (float)h[i];
             m[i] = (__bf16)rest;
             l[i] = (__bf16)(rest - (float)m[i]);
         }
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(largest) : "v"(hi[i]), "v"(hi[i + 1]));
         *reinterpret_cast<bf16x8*>(at) = h;
         *reinterpret_cast<bf16x8*>(at + plane_bytes) = m;
         *reinterpret_cast<bf16x8*>(at + 2 * plane_bytes) = l;
@@ -306,6 +302,26 @@ __device__ __forceinline__ void store_some(T* row, int q, int width, Value value
 #pragma unroll
         for (int e = 0; e < N; ++e)
             if (q + e < width) row[q + e] = o[e];
+    }
+}
+
+// s[k] += p(c) q(c, k) for c = 0 .. n - 1, one fp32 product after the other; only those of the bits `which` count, and once they are all NaN
+// they stay so.  Slow, and rare; its registers must not crowd the products before it, hence one element of the contraction at a time.
+template <int N, typename P, typename Q>
+__device__ __forceinline__ void plain_sums(int n, unsigned which, float (&s)[N], P p, Q q) {
+    static_assert(N <= 32, "");
+    for (int c0 = 0; c0 < n; c0 += 8) {
+        bool open = false;
+#pragma unroll
+        for (int k = 0; k < N; ++k) open |= (which >> k & 1) && !__builtin_isnan(s[k]);
+        if (!open) return;
+#pragma unroll 1
+        for (int c = c0; c < n && c < c0 + 8; ++c) {
+            const float x = p(c);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (which >> k & 1) s[k] = fmaf(x, q(c, k), s[k]);
+        }
     }
 }
 
@@ -446,7 +462,6 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         return (unsigned)r < (unsigned)rows ? r : -1;
     };
     Piece<T> hold_p[DMA ? 1 : NP], hold_q[DMA ? 1 : NQ];
-    float largest = 0.0f;
     int rest_p = 8, rest_q[kQCols ? 1 : NQ];  // "rows" in hold_*: elements before the contraction's end
     // dW: the rows of this lane's pieces, looked up before the pieces are asked for (both operands' pieces lie alike if BP == BQ)
     int row_p[kPCols ? NP : 1], row_q[kPCols && BP != BQ ? NQ : 1];
@@ -545,12 +560,12 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             if (!DMA && !kPCols && ragged) keep_first(hold_p[DMA ? 0 : n], rest_p);
-            store_piece(s + ((wave * NP + n) * 64 + lane) * 16, kPBytes, hold_p[DMA ? 0 : n], largest);
+            store_piece(s + ((wave * NP + n) * 64 + lane) * 16, kPBytes, hold_p[DMA ? 0 : n]);
         }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             if (!DMA && !kQCols && ragged) keep_first(hold_q[DMA ? 0 : n], rest_q[kQCols ? 0 : n]);
-            store_piece(s + F::kPlanes * kPBytes + ((wave * NQ + n) * 64 + lane) * 16, kQBytes, hold_q[DMA ? 0 : n], largest);
+            store_piece(s + F::kPlanes * kPBytes + ((wave * NQ + n) * 64 + lane) * 16, kQBytes, hold_q[DMA ? 0 : n]);
         }
     };
 
@@ -728,29 +743,27 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             barrier_lds_only();
         }
     }
+    auto plain_element = [&](const T* base, int64_t ld, int c, int col) {  // dW: column col of the run's row c; 0 where an index is out of range
+        const int r = a.order ? a.order[tl.first + c] : tl.first + c;
+        return (unsigned)r < (unsigned)rows ? (float)base[(int64_t)r * ld + col] : 0.0f;
+    };
+    uint64_t again = 0;  // fp32: this lane's sums that are not finite (see Frag<float>), bit (i FQ + j) 4 + e
     if constexpr (kWide) {
-        // an infinity among the operands: the sums again, element by element from memory (rare, and as slow as that sounds)
-        if (__syncthreads_or(__builtin_isinf(largest))) {
-            for (int i = 0; i < FP; ++i) {
-                const int p = pw + 16 * i + fr, row = kPCols ? 0 : rows_lds[p];
-                sumb[i] = accb[i] = 0.0f;
-                for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{};
-                if (kPCols ? p0 + p >= n_p : row < 0) continue;
-                for (int c = 0; c < n_c; ++c) {
-                    const int r = kPCols ? (a.order ? a.order[tl.first + c] : tl.first + c) : row;
-                    if ((unsigned)r >= (unsigned)rows) continue;
-                    const float x = P[(int64_t)r * a.ld_p + (kPCols ? p0 + p : c)];
-                    sumb[i] += kg == 0 ? x : 0.0f;
-                    for (int j = 0; j < FQ; ++j)
-                        for (int e = 0; e < 4; ++e) {
-                            const int q = q0 + qw + 16 * j + 4 * kg + e;
-                            if (q >= n_q) continue;
-                            const int64_t at = PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)(PRODUCT == kGradInput ? c : r) * a.ld_q + q;
-                            acc[i][j][e] = fmaf(x, Q[at], acc[i][j][e]);
-                        }
-                }
-            }
-        }
+        static_assert(FP * FQ * 4 <= 64 && FQ * 4 <= 16, "a bit for every sum");
+        float all = 0.0f;  // not finite if one of them is not
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) all += acc[i][j][e];
+        if (!__builtin_isfinite(all))
+#pragma unroll
+            for (int i = 0; i < FP; ++i)
+#pragma unroll
+                for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) again |= (uint64_t)!__builtin_isfinite(acc[i][j][e]) << ((i * FQ + j) * 4 + e);
     }
 
     // ---- lane: output row fr of P's fragment i, and of Q's fragments the columns column(j) .. + 3 (paired: of two, eight)
@@ -795,8 +808,40 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             v += __shfl_xor(v, 16);
             v += __shfl_xor(v, 32);
             if (kg != 0) continue;
+            if (kWide && !__builtin_isfinite(v)) {
+                float s[1] = {};
+                plain_sums(n_c, 1, s, [&](int c) { return plain_element(P, a.ld_p, c, p0 + p); }, [](int, int) { return 1.0f; });
+                v = s[0];
+            }
             if (a.chunk_rows) a.part[(int64_t)a.chunks * a.n_out * a.n_in + (int64_t)run * a.n_out + p0 + p] = v;
             else static_cast<T*>(a.dbias)[(int64_t)tl.g * a.n_out + p0 + p] = (T)v;
+        }
+    }
+    if constexpr (kWide) {
+        constexpr unsigned kRow = (1u << (FQ * 4)) - 1;
+        for (int i = 0; again; ++i, again >>= FQ * 4) {
+            const int p = pw + 16 * i + fr, row = kPCols ? p0 + p : rows_lds[p];
+            unsigned which = (unsigned)again & kRow;
+#pragma unroll
+            for (int k = 0; k < FQ * 4; ++k)
+                if (column(k >> 2) + (k & 3) >= n_q) which &= ~(1u << k);
+            if (!which || (kPCols ? row >= n_p : row < 0)) continue;
+            float s[FQ * 4] = {};
+            plain_sums(
+                n_c, which, s, [&](int c) { return kPCols ? plain_element(P, a.ld_p, c, row) : (float)P[(int64_t)row * a.ld_p + c]; },
+                [&](int c, int k) {
+                    const int q = column(k >> 2) + (k & 3);
+                    return PRODUCT == kGradWeight ? plain_element(Q, a.ld_q, c, q)
+                                                  : (float)Q[PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)c * a.ld_q + q];
+                });
+            float* const out = PRODUCT == kGradWeight ? (a.chunk_rows ? a.part : static_cast<float*>(a.out)) + ((int64_t)run * a.n_out + row) * a.n_in
+                               : a.splits > 1         ? a.part + ((int64_t)split * rows + row) * n_q
+                                                      : static_cast<float*>(a.out) + (int64_t)row * n_q;
+#pragma unroll
+            for (int k = 0; k < FQ * 4; ++k) {
+                const int q = column(k >> 2) + (k & 3);
+                if (which >> k & 1) out[q] = s[k] + (bias ? (float)bias[q] : 0.0f);
+            }
         }
     }
 }
@@ -835,7 +880,6 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
     const T* const P = static_cast<const T*>(a.p);
     const T* const W = static_cast<const T*>(a.q) + (none ? 0 : (int64_t)tl.g * a.n_in * a.n_out);
     float* const bias = reinterpret_cast<float*>(smem + PL * plane_bytes);
-    float largest = 0.0f;
 
     // ---- weights and bias -> LDS.  Piece (column, eight contraction elements): consecutive lanes take consecutive columns in dx (W's
     // rows are read along), consecutive chunks of a column in the forward pass
@@ -852,11 +896,11 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
         }
         const int in = col & 63, j = sizeof(T) == 4 ? in >> 4 : 2 * (in >> 5) + ((in >> 2) & 1);
         const int m = sizeof(T) == 4 ? in & 15 : 4 * ((in >> 3) & 3) + (in & 3);
-        store_piece(smem + ((((col >> 6) * 4 + j) * NC + (ch >> 2)) * 64 + (ch & 3) * 16 + m) * 16, plane_bytes, u, largest);
+        store_piece(smem + ((((col >> 6) * 4 + j) * NC + (ch >> 2)) * 64 + (ch & 3) * 16 + m) * 16, plane_bytes, u);
     }
     for (int i = t; i < blocks * 64; i += NT)
         bias[i] = PRODUCT == kForward && a.bias && !none && q0 + i < n_q ? (float)static_cast<const T*>(a.bias)[(int64_t)tl.g * a.n_out + q0 + i] : 0.0f;
-    const bool infinite = __syncthreads_or(__builtin_isinf(largest));
+    __syncthreads();
 
     auto row_of = [&](int first) { return first + fr < tl.last ? row_at(a, first + fr) : -1; };
     auto load_one = [&](int row, int k) {
@@ -885,7 +929,6 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
         row = row_next;
         T* const out = static_cast<T*>(a.out) + (int64_t)(out_row < 0 ? 0 : out_row) * n_q + q0;
         V p[sizeof(T) == 4 ? 1 : NC];
-        largest = 0.0f;
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int k = 0; k < NC; ++k) __builtin_memcpy(&p[k], u[k].v, 16);
@@ -906,7 +949,7 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
 #pragma unroll
                     for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(u[k].v[e]));
                     char planes[PL * 16];
-                    store_piece(planes, 16, u[k], largest);
+                    store_piece(planes, 16, u[k]);
                     if (b + 1 == blocks && more) {
                         int next = row;
                         asm volatile("" : "+v"(next));
@@ -923,21 +966,28 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
                         for (int j = 0; j < 4; ++j) acc[j] = F::mfma(*reinterpret_cast<const V*>(w + m * plane_bytes + (j * NC + k) * 1024), q[l], acc[j]);
                 if (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);  // (all k's splits and reads at once would not fit the registers)
             }
-            if (sizeof(T) == 4 && (infinite || __any(__builtin_isinf(largest)))) {  // an infinity: element by element (see Frag<float>)
-                for (int j = 0; j < 4; ++j)
-                    for (int e = 0; e < 4; ++e) {
-                        const int q = q0 + column(b, j) + e;
-                        float v = bias[q - q0];
-                        if (out_row >= 0 && q < n_q && !none)
-                            for (int c = 0; c < n_c; ++c)
-                                v = fmaf((float)P[(int64_t)out_row * a.ld_p + c], (float)W[PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)c * a.ld_q + q], v);
-                        acc[j][e] = v;
-                    }
-            }
             if (out_row < 0) continue;
             constexpr int kOnce = 16 / sizeof(T);
 #pragma unroll
             for (int j = 0; j < 4; j += kOnce / 4) store_some<T, kOnce>(out, column(b, j), width, [&](int e) { return acc[j + (e >> 2)][e & 3]; });
+            if constexpr (sizeof(T) == 4) {  // sums that are not finite (see Frag<float>)
+                float all = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) all += acc[k >> 2][k & 3];
+                if (__builtin_isfinite(all) || none) continue;
+                unsigned again = 0;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) again |= (unsigned)!__builtin_isfinite(acc[k >> 2][k & 3]) << k;
+                for (; again; again &= again - 1) {
+                    const int k = __ffs(again) - 1, in = column(b, k >> 2) + (k & 3), q = q0 + in;
+                    if (in >= width) continue;
+                    float s[1] = {bias[in]};
+                    plain_sums(
+                        n_c, 1, s, [&](int c) { return (float)P[(int64_t)out_row * a.ld_p + c]; },
+                        [&](int c, int) { return (float)W[PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)c * a.ld_q + q]; });
+                    out[in] = s[0];
+                }
+            }
         }
     }
 }
