@@ -2,7 +2,7 @@
 // never stored: what the fused kernels do between two linear layers (bayesian_ensemble.py:85-86), for any row width.
 //
 //   forward   y  = keep ? act(x) * s : 0            s = fp32(1 / (1-p)), act = ELU (alpha 1) or the identity
-//   backward  dx = keep ? dy * act'(x) * s : 0      act'(x) = x > 0 ? 1 : exp(x); the same mask drawn again
+//   backward  dx = keep ? dy * (act'(x) * s) : 0    act'(x) = x > 0 ? 1 : exp(x); the same mask drawn again
 //
 // keep of column c of row r: elem = elem_begin + c, block counter (((elem>>4)<<1) | ((elem>>2)&1), pair, 'MASK', row_begin + r),
 // slot = 4*((elem>>3)&1) + (elem&3) -> 16-bit half slot&1 of word slot>>1, kept iff it is < floor((1-p) * 65536)
@@ -105,8 +105,8 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(DropArgs a) {
             const uint32_t half = (j & 1) ? h[j >> 1] >> 16 : h[j >> 1] & 0xFFFFu;
             float v;
             if (BACKWARD) {
-                v = g[i][j] * a.scale;
-                if (ELU) v *= x[i][j] > 0.0f ? 1.0f : __expf(x[i][j]);
+                // (the factors first: dy * s alone may overflow where the result does not)
+                v = g[i][j] * (ELU ? a.scale * (x[i][j] > 0.0f ? 1.0f : __expf(x[i][j])) : a.scale);
             } else {
                 v = x[i][j];
                 if (ELU) v = v > 0.0f ? v : elu_neg(v);

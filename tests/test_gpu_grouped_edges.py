@@ -3,9 +3,9 @@ n products kept in 32 bits is off by at most n * 2^-23 * sum|a||b|, the result b
 import pytest
 import torch
 
-from grouped_checks import U, agree_as_fp32
+from grouped_checks import U, agree, agree_as_fp32
 from mcmc_amd import grouped_linear
-from test_gpu_grouped import DEV, FP32, linear_case, run_linear
+from test_gpu_grouped import BF16, DEV, FP32, dropout_reference, keep_flags, linear_case, run_dropout, run_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,16 @@ def test_fp32_products_at_the_top_of_the_range(big, R, G, K, N, ordered):
     got = run_linear(xs, w, b, ds, groups)
     agree_as_fp32(got["dw"], refw, refw.abs() * 2 * U, "dw")
     agree_as_fp32(got["db"], refb, refb.abs() * U, "db")
+
+
+@pytest.mark.parametrize("p", [0.1, 0.5, 0.9])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_dropout_gradient_where_only_a_factor_overflows(dtype, p):
+    """dy / (1 - p) is beyond fp32, dy * elu'(x) / (1 - p) is not: x from -3 down to where exp(x) is 0."""
+    x = -torch.linspace(3, 200, 64 * 24, device=DEV).view(64, 24).to(dtype)
+    dy = torch.full_like(x, 3.3e38)
+    dy[:, ::2] *= -1
+    got = run_dropout(x, dy, p, 21, activation="elu")
+    ref = dropout_reference(x, dy, keep_flags(21, 0, 64, 24, p), p, "elu")
+    assert got["dx"].isfinite().all()
+    agree(got["dx"], *ref["dx"], "dx")
