@@ -10,9 +10,10 @@ product runs over the ragged groups in one launch:
     y = grouped_linear(h, w_out, groups, b_out)
 
 All arithmetic is in libmcmc_hip.so (``mcmc_group_rows``, ``mcmc_grouped_linear_*``, ``mcmc_dropout_*``); gradients are ordinary
-autograd.  There is no CPU path.  Every call runs on the current stream of its tensors' device and allocates what it needs from
-torch, nothing is kept from one call for the next, so calls may be captured into HIP graphs (after a first call outside the
-capture, which loads the kernels; a backward pass, as torch has it, only while no eager graph of the same leaves is alive).
+autograd, of the first order and in reverse mode (other derivatives are refused).  There is no CPU path.  Every call runs on the
+current stream of its tensors' device and allocates what it needs from torch, nothing is kept from one call for the next, so calls
+may be captured into HIP graphs (after a first call outside the capture, which loads the kernels; a backward pass, as torch has
+it, only while no eager graph of the same leaves is alive).
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ from contextlib import nullcontext
 from typing import NamedTuple, Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -82,18 +84,26 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
 
 
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """A forward-mode tangent does not show in requires_grad, and holds whatever the grad mode."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _once(backward):
     """Gradients of gradients are refused like once_differentiable does it, but its bookkeeping (20 us a call) is paid only by a
-    backward pass that records a graph."""
+    backward pass that records a graph; so are tangents of dy."""
     recorded = once_differentiable(backward)
 
     def run(ctx, dy):
+        if _has_tangent(dy):
+            raise NotImplementedError("the gradients of mcmc_amd's grouped operators have no forward-mode derivative (jvp)")
         return recorded(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
     return run
 
 
 def _wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether the call has to pass through autograd: for a gradient, or to be refused there (no operator has a jvp)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or _has_tangent(*tensors)
 
 
 class RowGroups(NamedTuple):

@@ -1,0 +1,45 @@
+"""CPU-only tests of the grouped operators: calls that are refused, with the launches stubbed where a refusal comes after them."""
+from contextlib import nullcontext
+from types import SimpleNamespace
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from mcmc_amd import RowGroups, grouped, grouped_linear, philox_dropout
+
+
+@pytest.fixture
+def no_device(monkeypatch):
+    """The operators' Python on CPU tensors: no device is looked for, nothing is launched, results are zeros."""
+    monkeypatch.setattr(grouped, "_engine", lambda *a, **kw: SimpleNamespace())
+    monkeypatch.setattr(grouped, "_on", lambda eng: nullcontext())
+    monkeypatch.setattr(grouped, "_workspace_bytes", lambda *a: 0)
+    monkeypatch.setattr(grouped, "_forward", lambda eng, x, w, b, order, offsets: x.new_zeros(x.shape[0], w.shape[1]))
+    monkeypatch.setattr(grouped, "_dropout", lambda eng, x, args: (torch.zeros_like(x), x))
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "dropout"])
+def test_forward_mode_derivatives_are_refused(no_device, which, grad_mode):
+    """A tangent does not show in requires_grad; without a look for it the derivative would be zero without a word."""
+    args = {"x": torch.ones(4, 3), "weight": torch.ones(2, 5, 3), "bias": torch.ones(2, 5)}
+    groups = RowGroups(None, torch.tensor([0, 2, 4], dtype=torch.int32))
+    with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+        assert grouped_linear(args["x"], args["weight"], groups, args["bias"]).shape == (4, 5)  # no tangent: an ordinary call
+        with pytest.raises(NotImplementedError, match="jvp"):
+            if which == "dropout":
+                philox_dropout(forward_ad.make_dual(args["x"], torch.ones(4, 3)), 0.1, 1)
+            else:
+                args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+                grouped_linear(args["x"], args["weight"], groups, args["bias"])
+
+
+@pytest.mark.parametrize("which", ["linear", "dropout"])
+def test_tangents_of_the_output_gradient_are_refused(no_device, which):
+    x, groups = torch.ones(4, 3, requires_grad=True), RowGroups(None, torch.tensor([0, 2, 4], dtype=torch.int32))
+    y = philox_dropout(x, 0.1, 1) if which == "dropout" else grouped_linear(x, torch.ones(2, 5, 3), groups)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            torch.autograd.grad(y, x, dual)
