@@ -5,7 +5,8 @@ import torch
 
 from grouped_checks import U, agree, agree_as_fp32
 from mcmc_amd import grouped_linear
-from test_gpu_grouped import BF16, DEV, FP32, dropout_reference, keep_flags, linear_case, run_dropout, run_linear
+from test_gpu_grouped import (BF16, DEV, FP16, FP32, SIZES, dropout_reference, gen, keep_flags, linear_case, linear_reference, run_dropout,
+                              run_linear)
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +77,113 @@ def test_dropout_gradient_where_only_a_factor_overflows(dtype, p):
     ref = dropout_reference(x, dy, keep_flags(21, 0, 64, 24, p), p, "elu")
     assert got["dx"].isfinite().all()
     agree(got["dx"], *ref["dx"], "dx")
+
+
+# ------------------------------------------------------------------------------------------------- one product a sum
+ONE_HOT = [(300, 3, 11, 256), (400, 3, 64, 128), (400, 3, 128, 64), (600, 3, 256, 128), (1000, 3, 300, 200), (1000, 2, 200, 300), (1100, 2, 513, 1031),
+           (2100, 2, 2048, 64), (2100, 2, 64, 2048), (16_700, 3, 1032, 1024), (4200, 2, 2048, 2056), (60_000, 3, 64, 48), (30_011, 5, 11, 256),
+           (20_000, 2, 64, 1)]
+
+
+def all_bits(dtype, shape, g):
+    """Random signs, exponents 0 .. 3 and mantissas of every bit the type has, the last one set: no plane of an fp32 value is 0 for many."""
+    bits = {FP32: 24, BF16: 8, FP16: 11}[dtype]
+    m = torch.randint(2 ** (bits - 2), 2 ** (bits - 1), shape, generator=g, device=DEV) * 2 + 1
+    e = torch.randint(0, 4, shape, generator=g, device=DEV) - (bits - 1)
+    s = torch.randint(0, 2, shape, generator=g, device=DEV) * 2 - 1
+    return (m.double() * s * torch.exp2(e.double())).to(dtype)
+
+
+def powers(dtype, shape, g):
+    return (torch.exp2(torch.randint(-2, 3, shape, generator=g, device=DEV).float()) * (torch.randint(0, 2, shape, generator=g, device=DEV) * 2 - 1)).to(dtype)
+
+
+def same(got, ref, what):
+    assert torch.equal(got, ref.to(got.dtype)), f"{what}: {int((got != ref.to(got.dtype)).sum())} of {ref.numel()} off"
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", ONE_HOT)
+def test_one_product_a_sum(R, G, K, N, dtype):
+    """Operands with all their bits, one product in every sum, at every place of the contraction: 16-bit products are exact in fp32, and so
+    are fp32 ones with a power of two, whichever side it is on; of two full fp32 operands the sum is their product within 2 u."""
+    x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, 820)
+    g, rows, zero = gen(821), torch.arange(R, device=DEV), torch.zeros_like(b)
+    for left, right in ((all_bits, powers), (powers, all_bits), (all_bits, all_bits)):
+        def close(got, ref, what):
+            if dtype == FP32 and left is right:
+                agree(got, ref, ref.abs() * 2 * U, what)
+            else:
+                same(got, ref, what)
+        w = right(dtype, (G, N, K), g)
+        mine = left(dtype, (R,), g)
+        xs, ds = torch.zeros_like(x), torch.zeros_like(dy)
+        xs[rows, rows % K], ds[rows, rows % N] = mine, mine
+        close(grouped_linear(xs, w, groups, zero), mine.double()[:, None] * w.double()[ids, :, rows % K], "y")
+        close(run_linear(xs, w, zero, ds, groups)["dx"], mine.double()[:, None] * w.double()[ids, rows % N], "dx")
+        for trial in range(3):  # dW: column n of dy has one row
+            xs, ds = left(dtype, (R, K), g), torch.zeros_like(dy)
+            dw, db = torch.zeros(G, N, K, device=DEV, dtype=torch.float64), torch.zeros(G, N, device=DEV, dtype=torch.float64)
+            for i in range(G):
+                of = (ids == i).nonzero()[:, 0]
+                n = min(N, of.numel())
+                at = torch.randperm(of.numel(), generator=g, device=DEV)[:n]
+                at[:2] = torch.tensor([of.numel() - 1, 0], device=DEV)[:n] if trial == 0 else at[:2]
+                at, n = (at.unique(), at.unique().numel())
+                r, cols, v = of[at], torch.arange(n, device=DEV), right(dtype, (n,), g)
+                ds[r, cols] = v
+                dw[i, :n], db[i, :n] = v.double()[:, None] * xs[r].double(), v.double()
+            got = run_linear(xs, w, b, ds, groups)
+            close(got["dw"], dw, "dw")
+            same(got["db"], db, "db")
+
+
+# ------------------------------------------------------------------------------------------ nothing else reaches a result
+EVERYWHERE = SIZES + [(60_000, 3, 64, 48), (20_000, 9, 64, 1), (9000, 1, 200, 136), (3001, 3, 1000, 520), (600, 2, 2048, 2056), (8, 2, 4096, 512),
+                      (5, 2, 2193, 10), (300, 9, 3, 3634), (16_700, 3, 1032, 1024), (4200, 16, 1032, 1000)]
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", EVERYWHERE)
+def test_results_are_finite_and_near(R, G, K, N, dtype):
+    """Every product in every kernel, where a NaN is off like any other wrong value."""
+    for ordered, stray in ((False, 0.1), (True, 0.0)):
+        x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, R + 2 * K, ordered, stray)
+        got = run_linear(x, w, b, dy, groups)
+        ref, mag = linear_reference(x, w, b, dy, ids)
+        for n in ref:
+            agree(got[n], ref[n], mag[n] * U, f"{n} ordered={ordered}")
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", [s for s in EVERYWHERE if s[1] >= 3 and s[0] >= 37])
+def test_foreign_nan_and_infinities_stay_outside(R, G, K, N, dtype):
+    """Rows of no group hold NaN and infinities, and so do the rows, the weights and the bias of group 1: the other groups' results are those
+    of clean operands."""
+    x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, 31 + R, stray=0.1)
+    clean = [t.clone() for t in (x, w, b, dy)]
+    own, out = ids == 1, ids < 0
+    clean[0][out | own], clean[3][out | own], clean[1][1], clean[2][1] = 0, 0, 0, 0
+    ref, mag = linear_reference(*clean, ids)
+    others = [i for i in range(G) if i != 1]
+    for bad, worse in ((float("nan"), float("inf")), (-float("inf"), float("nan"))):
+        x, w, b, dy = (t.clone() for t in clean)
+        x[out], dy[out], x[own], dy[own], w[1], b[1] = bad, worse, worse, bad, worse, bad
+        got = run_linear(x, w, b, dy, groups)
+        for n in ("y", "dx"):
+            assert not got[n][out].any(), n
+            agree(got[n][~own], ref[n][~own], mag[n][~own] * U, n)
+        for n in ("dw", "db"):
+            agree(got[n][others], ref[n][others], mag[n][others] * U, n)
+        assert got["y"][own].isnan().all() and (got["dw"][1].isnan().all() or not own.any())
+
+
+@pytest.mark.parametrize("act", [None, "elu"])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("rows, width, p", [(1, 1, 0.1), (5, 8, 0.1), (33, 64, 0.0), (4, 1001, 0.25), (700, 24, 0.9), (1000, 17, 0.1)])
+def test_dropout_is_finite_and_near(rows, width, p, dtype, act):
+    x = (torch.randn(rows, width, generator=gen(rows), device=DEV) * 2).to(dtype)
+    dy = torch.randn(rows, width, generator=gen(width), device=DEV).to(dtype)
+    got, ref = run_dropout(x, dy, p, 77 + rows, activation=act, pair=3), dropout_reference(x, dy, keep_flags(77 + rows, 3, rows, width, p), p, act)
+    for n in ("y", "dx"):
+        agree(got[n], *ref[n], n)

@@ -6,6 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from grouped_checks import agree, agree_as_fp32
 from mcmc_amd import RowGroups, grouped, grouped_linear, philox_dropout
 
 
@@ -43,3 +44,18 @@ def test_tangents_of_the_output_gradient_are_refused(no_device, which):
         dual = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(NotImplementedError, match="jvp"):
             torch.autograd.grad(y, x, dual)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 1.1])
+def test_the_comparison_sees_every_wrong_value(bad):
+    one, slack = torch.ones(3, dtype=torch.float64), torch.full((3,), 1e-3, dtype=torch.float64)
+    agree(torch.ones(3), one, slack, "ones")
+    got = torch.tensor([1.0, bad, 1.0])
+    for check in (agree, agree_as_fp32):
+        with pytest.raises(AssertionError, match="1 of 3 off"):
+            check(got, one, slack, "one of them")
+    for ref, tol in ((one / 0, slack), (one, slack / 0)):
+        with pytest.raises(AssertionError, match="not finite"):
+            agree(torch.ones(3), ref, tol, "a mistake of the test")
+    with pytest.raises(AssertionError, match="infinities"):
+        agree_as_fp32(torch.full((3,), 3e38), one * 1e39, slack, "beyond fp32")
