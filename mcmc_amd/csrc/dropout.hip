@@ -32,7 +32,7 @@ struct DropArgs {
     const void* dy;  // backward
     void* out;
     int64_t ld_x, ld_dy, ld_out;  // elements between rows
-    int64_t units;                // rows * units_per_row
+    int64_t units;                // rows of this launch * units_per_row
     uint32_t units_per_row, width;
     uint64_t seed;
     const uint64_t* seed_dev;     // not NULL: the key is read when the kernel runs
@@ -118,16 +118,27 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(DropArgs a) {
     }
 }
 
+// A launch counts its threads in 32 bits: larger calls go row by row in pieces of at most 2^31 threads (2^32 units, at least 16 rows)
+constexpr int64_t kMostUnits = (int64_t)1 << 32;
+
 template <typename T>
-int launch(const DropArgs& a, bool elu, bool backward, hipStream_t s) {
-    const int64_t blocks = (a.units + kThreads * kUnits - 1) / (kThreads * kUnits);
-    MCMC_REQUIRE(blocks <= 0x7FFFFFFFLL, "rows * width is too large for one call (%lld workgroups)", (long long)blocks);
-    const dim3 grid((unsigned)blocks);
-    if (elu && backward) dropout_kernel<T, true, true><<<grid, kThreads, 0, s>>>(a);
-    else if (elu) dropout_kernel<T, true, false><<<grid, kThreads, 0, s>>>(a);
-    else if (backward) dropout_kernel<T, false, true><<<grid, kThreads, 0, s>>>(a);
-    else dropout_kernel<T, false, false><<<grid, kThreads, 0, s>>>(a);
-    return check_launch("dropout_kernel");
+int launch(DropArgs a, int64_t rows, bool elu, bool backward, hipStream_t s) {
+    const int64_t most = kMostUnits / a.units_per_row;
+    for (; rows > 0; rows -= most) {
+        a.units = (rows < most ? rows : most) * (int64_t)a.units_per_row;
+        const dim3 grid((unsigned)((a.units + kThreads * kUnits - 1) / (kThreads * kUnits)));
+        if (elu && backward) dropout_kernel<T, true, true><<<grid, kThreads, 0, s>>>(a);
+        else if (elu) dropout_kernel<T, true, false><<<grid, kThreads, 0, s>>>(a);
+        else if (backward) dropout_kernel<T, false, true><<<grid, kThreads, 0, s>>>(a);
+        else dropout_kernel<T, false, false><<<grid, kThreads, 0, s>>>(a);
+        if (int rc = check_launch("dropout_kernel")) return rc;
+        if (rows <= most) break;
+        if (a.x) a.x = static_cast<const T*>(a.x) + most * a.ld_x;
+        if (a.dy) a.dy = static_cast<const T*>(a.dy) + most * a.ld_dy;
+        a.out = static_cast<T*>(a.out) + most * a.ld_out;
+        a.row_begin += (uint32_t)most;
+    }
+    return MCMC_OK;
 }
 
 }  // namespace
@@ -143,7 +154,6 @@ int launch_dropout(int dtype, bool elu, bool backward, const void* x, int64_t ld
     a.ld_dy = ld_dy;
     a.ld_out = ld_out;
     a.units_per_row = 2 * (uint32_t)((width + 15) / 16);
-    a.units = rows * (int64_t)a.units_per_row;
     a.width = (uint32_t)width;
     a.seed = seed;
     a.seed_dev = seed_dev;
@@ -152,9 +162,9 @@ int launch_dropout(int dtype, bool elu, bool backward, const void* x, int64_t ld
     a.row_begin = row_begin;
     a.block_begin = (elem_begin >> 4) << 1;
     a.scale = (float)(1.0 / (1.0 - (double)p_drop));
-    if (dtype == MCMC_DT_F32) return launch<float>(a, elu, backward, s);
-    if (dtype == MCMC_DT_BF16) return launch<__bf16>(a, elu, backward, s);
-    return launch<_Float16>(a, elu, backward, s);
+    if (dtype == MCMC_DT_F32) return launch<float>(a, rows, elu, backward, s);
+    if (dtype == MCMC_DT_BF16) return launch<__bf16>(a, rows, elu, backward, s);
+    return launch<_Float16>(a, rows, elu, backward, s);
 }
 
 }  // namespace mcmc

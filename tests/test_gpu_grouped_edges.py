@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from grouped_checks import U, agree, agree_as_fp32
-from mcmc_amd import grouped_linear
+from mcmc_amd import grouped_linear, philox_dropout
 from test_gpu_grouped import (BF16, DEV, FP16, FP32, SIZES, dropout_reference, gen, keep_flags, linear_case, linear_reference, run_dropout,
                               run_linear)
 
@@ -77,6 +77,21 @@ def test_dropout_gradient_where_only_a_factor_overflows(dtype, p):
     ref = dropout_reference(x, dy, keep_flags(21, 0, 64, 24, p), p, "elu")
     assert got["dx"].isfinite().all()
     agree(got["dx"], *ref["dx"], "dx")
+
+
+@pytest.mark.parametrize("width", [1, 17])
+def test_dropout_of_more_rows_than_a_launch_has_threads(width):
+    """As many rows as the counter can name (17 columns: a third of them), forward and backward: around every 2^30th row and at the end
+    the result is that of the rows alone."""
+    R = 2 ** 32 if width == 1 else 2 ** 32 // 3
+    x = torch.tensor([[1.5]], device=DEV, dtype=FP16).expand(R, width).requires_grad_()
+    y = philox_dropout(x, 0.3, 55, pair=2)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    for at in list(range(0, R, 2 ** 30)) + [R - 64]:
+        first, last = max(0, at - 64), min(R, at + 64)
+        alone = philox_dropout(x.detach()[first:last], 0.3, 55, pair=2, row_begin=first)
+        assert torch.equal(y.detach()[first:last], alone) and torch.equal(dx[first:last], alone), at
+        assert torch.equal(alone != 0, keep_flags(55, 2, last - first, width, 0.3, row_begin=first)), at
 
 
 # ------------------------------------------------------------------------------------------------- one product a sum
