@@ -428,7 +428,9 @@ int mcmc_tft_adamw(mcmc_ctx* ctx, float* P, float* PT, int num_features, const f
 /* ---- operators over ragged groups of rows ---------------------------------------------------- */
 /* The reference hands every member the whole batch (bayesian_ensemble.py:160-169); these serve members (or experts) that each own
  * a different share of the rows, and layers of any width.  Limits: rows <= MCMC_GROUPED_MAX_ROWS; n_groups, n_in and n_out in
- * [1, MCMC_GROUPED_MAX_DIM].
+ * [1, MCMC_GROUPED_MAX_DIM].  mcmc_grouped_linear_forward and _grad_input walk all offsets in every workgroup: their time grows with
+ * n_groups times rows once there are thousands of groups, and calls that would walk for more than a few seconds (2^20 groups of one row
+ * each, 2^27 groups of any rows) are refused, by mcmc_grouped_linear_workspace_bytes too.
  *
  * mcmc_group_rows: the rows sorted stably by group.
  *   ids     [rows] int32 (id_bytes 4) or int64 (8): the row's group; a value outside 0..n_groups-1 = no group

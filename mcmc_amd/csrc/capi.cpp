@@ -760,7 +760,9 @@ int64_t mcmc_grouped_linear_workspace_bytes(int product, int dtype, int64_t rows
 }
 
 static int check_grouped_workspace(int product, int dtype, int64_t rows, int n_groups, int n_in, int n_out, const void* workspace) {
-    if (grouped_linear_workspace_bytes(product, dtype, rows, n_groups, n_in, n_out) > 0)
+    const int64_t bytes = grouped_linear_workspace_bytes(product, dtype, rows, n_groups, n_in, n_out);
+    if (bytes < 0) return (int)bytes;
+    if (bytes > 0)
         MCMC_REQUIRE(workspace && aligned16(workspace), "workspace must be 16-byte aligned device memory (mcmc_grouped_linear_workspace_bytes)");
     return MCMC_OK;
 }

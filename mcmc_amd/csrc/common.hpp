@@ -157,6 +157,7 @@ int launch_grouped_linear_forward(int dtype, const void* x, int64_t ld_x, int64_
                                   int n_out, const void* weight, const void* bias, void* y, void* ws, hipStream_t s);
 int launch_grouped_linear_grad_input(int dtype, const void* dy, int64_t ld_dy, int64_t rows, const int* order, const int* offsets, int G, int n_in,
                                      int n_out, const void* weight, void* dx, void* ws, hipStream_t s);
+// < 0: an error, for calls that are refused
 int64_t grouped_linear_workspace_bytes(int product, int dtype, int64_t rows, int G, int n_in, int n_out);
 int launch_grouped_linear_grad_weight(int dtype, const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int64_t rows, const int* order,
                                       const int* offsets, int G, int n_in, int n_out, void* dweight, void* dbias, void* ws, hipStream_t s);

@@ -1190,8 +1190,8 @@ int chunk_rows_of(int64_t rows, int G, int n_in, int n_out) {
 }
 int chunks_of(int64_t rows, int G, int per) { return (int)(rows / per + (G < rows ? G : rows)); }
 
-int check_grid(int64_t blocks) {
-    MCMC_REQUIRE(blocks <= 0x7FFFFFFFLL, "rows, groups and widths are too large for one call (%lld workgroups)", (long long)blocks);
+int check_grid(int64_t blocks, int threads) {  // a launch counts its threads in 32 bits
+    MCMC_REQUIRE(blocks * threads <= 0xFFFFFFFFLL, "rows, groups and widths are too large for one call (%lld workgroups)", (long long)blocks);
     return MCMC_OK;
 }
 
@@ -1242,25 +1242,34 @@ int launch_strip_n(const Args& a, int q_tile, int run, unsigned blocks, hipStrea
     return check_launch("grouped_strip_kernel");
 }
 
-template <typename T, int PRODUCT>
-int launch_strip(const Args& a, int q_tile, hipStream_t s) {
-    const int n_q = PRODUCT == kForward ? a.n_out : a.n_in, n_c = PRODUCT == kForward ? a.n_in : a.n_out;
-    // Rows per workgroup, whole turns of its waves: eight times the bytes of its weights in LDS and 4 KB, for what it costs to start (a workgroup
-    // with fewer rows spends its time there, one with more leaves a long tail: 1,048,576 rows 11 -> 256 bf16: 1,024 rows 205 us, 256 rows 161; 256 -> 11
-    // fp32: 200 and 264), but no fewer workgroups than 1,024 as long as each has a turn.
+struct Strip {
+    int run;         // rows per workgroup
+    int64_t blocks;
+};
+// Rows per workgroup, whole turns of its waves: eight times the bytes of its weights in LDS and 4 KB, for what it costs to start (a workgroup
+// with fewer rows spends its time there, one with more leaves a long tail: 1,048,576 rows 11 -> 256 bf16: 1,024 rows 205 us, 256 rows 161; 256 -> 11
+// fp32: 200 and 264), but no fewer workgroups than 1,024 as long as each has a turn.
+template <typename T>
+Strip strip_of(int64_t rows, int G, int n_c, int n_q, int q_tile) {
     const int nc = n_c <= 32 ? 1 : n_c <= 64 ? 2 : n_c <= 128 ? 4 : 8;
     const int64_t weights = (int64_t)nc * 64 * Frag<T>::kPlanes * q_tile, row = (int64_t)sizeof(T) * (n_c + (n_q < q_tile ? n_q : q_tile));
     constexpr int kTurn = 16 * kStripWaves;
     int64_t run = 8 * (weights + 4096) / row;
-    run = a.rows / 1024 < run ? a.rows / 1024 : run;
+    run = rows / 1024 < run ? rows / 1024 : run;
     run = run / kTurn * kTurn;
     run = run < kTurn ? kTurn : run;
-    const int64_t blocks = (a.rows / run + (a.G + 1 < a.rows ? a.G + 1 : a.rows)) * ceil_div(n_q, q_tile);
-    if (int rc = check_grid(blocks)) return rc;
-    if (nc == 1) return launch_strip_n<T, PRODUCT, 1>(a, q_tile, (int)run, (unsigned)blocks, s);
-    if (nc == 2) return launch_strip_n<T, PRODUCT, 2>(a, q_tile, (int)run, (unsigned)blocks, s);
-    if (nc == 4) return launch_strip_n<T, PRODUCT, 4>(a, q_tile, (int)run, (unsigned)blocks, s);
-    return launch_strip_n<T, PRODUCT, 8>(a, q_tile, (int)run, (unsigned)blocks, s);
+    return Strip{(int)run, (rows / run + (G + 1 < rows ? G + 1 : rows)) * ceil_div(n_q, q_tile)};
+}
+
+template <typename T, int PRODUCT>
+int launch_strip(const Args& a, int q_tile, hipStream_t s) {
+    const int n_q = PRODUCT == kForward ? a.n_out : a.n_in, n_c = PRODUCT == kForward ? a.n_in : a.n_out;
+    const Strip p = strip_of<T>(a.rows, a.G, n_c, n_q, q_tile);
+    if (int rc = check_grid(p.blocks, 64 * kStripWaves)) return rc;
+    if (n_c <= 32) return launch_strip_n<T, PRODUCT, 1>(a, q_tile, p.run, (unsigned)p.blocks, s);
+    if (n_c <= 64) return launch_strip_n<T, PRODUCT, 2>(a, q_tile, p.run, (unsigned)p.blocks, s);
+    if (n_c <= 128) return launch_strip_n<T, PRODUCT, 4>(a, q_tile, p.run, (unsigned)p.blocks, s);
+    return launch_strip_n<T, PRODUCT, 8>(a, q_tile, p.run, (unsigned)p.blocks, s);
 }
 
 // Parts of a long contraction (forward, dx) where the output has too few tiles to fill the chip: a step of one workgroup waits for
@@ -1281,6 +1290,20 @@ Split split_of(int product, int64_t rows, int G, int n_in, int n_out) {
     return Split{ceil_div(n_c, c), c};
 }
 
+// From 64 groups on every workgroup of a forward or dx product walks the offsets, 64 groups a step of 0.3 us, twice: with as many groups as
+// rows the time grows with their square (64 -> 64 bf16: 4,096 groups, 8,192 rows 0.25 ms; 65,536 and 65,536 rows 56 ms; 2^20 and 2^20 would
+// take 14 s).  What would take more than a few seconds is refused; 4,096 workgroups count as the least, which one walk takes as well.
+template <typename T>
+int check_walks(int product, int64_t rows, int G, int n_in, int n_out) {
+    if (product == kGradWeight || G < 64 || rows == 0) return MCMC_OK;
+    const int n_c = product == kForward ? n_in : n_out, n_q = product == kForward ? n_out : n_in, q_tile = strip_q_tile<T>(n_c, n_q);
+    int64_t blocks = q_tile ? strip_of<T>(rows, G, n_c, n_q, q_tile).blocks
+                            : (rows / 128 + (G + 1 < rows ? G + 1 : rows)) * ceil_div(n_q, 128) * split_of<T>(product, rows, G, n_in, n_out).parts;
+    blocks = blocks < 4096 ? 4096 : blocks;
+    MCMC_REQUIRE(blocks <= ((int64_t)1 << 38) / G, "%d groups are too many for %lld rows: their offsets would be searched for seconds", G, (long long)rows);
+    return MCMC_OK;
+}
+
 template <typename T>
 int launch(int product, Args a, hipStream_t s) {
     const int n_q = product == kForward ? a.n_out : a.n_in;
@@ -1296,21 +1319,21 @@ int launch(int product, Args a, hipStream_t s) {
     const int64_t runs = product == kGradWeight ? (int64_t)ceil_div(a.n_out, sh.bp) * (a.chunk_rows ? a.chunks : a.G)
                                                 : (a.rows / sh.bp + (a.G + 1 < a.rows ? a.G + 1 : a.rows)) * a.splits;
     const int64_t blocks = runs * ceil_div(n_q, sh.bq);
-    if (int rc = check_grid(blocks)) return rc;
+    if (int rc = check_grid(blocks, sh.bp == 256 ? 512 : 256)) return rc;
     if (product != kGradWeight) {
         if (int rc = product == kForward ? launch_product<T, kForward>(a, sh, dma, (unsigned)blocks, s)
                                          : launch_product<T, kGradInput>(a, sh, dma, (unsigned)blocks, s))
             return rc;
         if (a.splits == 1) return MCMC_OK;
         const int64_t n = a.rows * n_q, joins = (n + kThreads - 1) / kThreads;
-        if (int rc = check_grid(joins)) return rc;
+        if (int rc = check_grid(joins, kThreads)) return rc;
         grouped_join_kernel<T><<<(unsigned)joins, kThreads, 0, s>>>(a.part, a.splits, n, static_cast<T*>(a.out));
         return check_launch("grouped_join_kernel");
     }
     const bool thin_out = a.n_out <= kThinMost;
     if (thin_out || a.n_in < kThinMost) {
         const int64_t thin = (int64_t)ceil_div(thin_out ? a.n_in : a.n_out, kThinCols) * (a.chunk_rows ? a.chunks : a.G);
-        if (int rc = check_grid(thin)) return rc;
+        if (int rc = check_grid(thin, 256)) return rc;
         if (thin_out) grouped_thin_kernel<T, true><<<(unsigned)thin, 256, 0, s>>>(a);
         else grouped_thin_kernel<T, false><<<(unsigned)thin, 256, 0, s>>>(a);
         if (int rc = check_launch("grouped_thin_kernel")) return rc;
@@ -1322,7 +1345,7 @@ int launch(int product, Args a, hipStream_t s) {
     // in all, 65 with one thread; up to 64 chunks the same)
     const int slices = a.chunks / a.G > 16 ? 8 : 1;
     const int64_t sums = ((int64_t)a.n_out * a.n_in + (a.dbias ? a.n_out : 0) + kThreads / slices - 1) / (kThreads / slices) * a.G;
-    if (int rc = check_grid(sums)) return rc;
+    if (int rc = check_grid(sums, kThreads)) return rc;
     if (slices == 8) grouped_sum_kernel<T, 8><<<(unsigned)sums, kThreads, 0, s>>>(a);
     else grouped_sum_kernel<T, 1><<<(unsigned)sums, kThreads, 0, s>>>(a);
     return check_launch("grouped_sum_kernel");
@@ -1348,12 +1371,15 @@ int launch_grouped_linear_grad_input(int dtype, const void* dy, int64_t ld_dy, i
                         Args{dy, weight, nullptr, dx, nullptr, static_cast<float*>(ws), order, offsets, ld_dy, n_in, rows, G, n_in, n_out, 0, 0, 1, 0}, s);
 }
 
+// < 0: an error, for calls that are refused
 int64_t grouped_linear_workspace_bytes(int product, int dtype, int64_t rows, int G, int n_in, int n_out) {
     if (product == kGradWeight) {
         const int per = chunk_rows_of(rows, G, n_in, n_out);
         return per ? (int64_t)chunks_of(rows, G, per) * ((int64_t)n_in + 1) * n_out * 4 : 0;
     }
-    const Split split = dtype == MCMC_DT_F32 ? split_of<float>(product, rows, G, n_in, n_out) : split_of<__bf16>(product, rows, G, n_in, n_out);
+    const bool wide = dtype == MCMC_DT_F32;
+    if (int rc = wide ? check_walks<float>(product, rows, G, n_in, n_out) : check_walks<__bf16>(product, rows, G, n_in, n_out)) return rc;
+    const Split split = wide ? split_of<float>(product, rows, G, n_in, n_out) : split_of<__bf16>(product, rows, G, n_in, n_out);
     return split.parts > 1 ? (int64_t)split.parts * rows * (product == kForward ? n_out : n_in) * 4 : 0;
 }
 

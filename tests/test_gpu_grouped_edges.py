@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from grouped_checks import U, agree, agree_as_fp32
-from mcmc_amd import grouped_linear, philox_dropout
+from mcmc_amd import RowGroups, grouped_linear, philox_dropout
 from test_gpu_grouped import (BF16, DEV, FP16, FP32, SIZES, dropout_reference, gen, keep_flags, linear_case, linear_reference, run_dropout,
                               run_linear)
 
@@ -202,3 +202,49 @@ def test_dropout_is_finite_and_near(rows, width, p, dtype, act):
     got, ref = run_dropout(x, dy, p, 77 + rows, activation=act, pair=3), dropout_reference(x, dy, keep_flags(77 + rows, 3, rows, width, p), p, act)
     for n in ("y", "dx"):
         agree(got[n], *ref[n], n)
+
+
+# ---------------------------------------------------------------------------------------------------------- many groups
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", [(8192, 4096, 64, 64), (3000, 5000, 16, 24), (2500, 1000, 300, 130), (9, 65, 2048, 64), (9, 65, 64, 2048),
+                                        (20_000, 130, 64, 48), (3, 70_000, 5, 6), (700, 64, 40, 33), (700, 63, 40, 33)])
+def test_more_groups_than_a_wave_has_lanes(R, G, K, N, dtype):
+    """63, 64 and more groups, most of them short or empty, rows of no group among them."""
+    for ordered in (False, True):
+        x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, 900 + G, ordered, 0.1) if G <= 4096 else many_groups(R, G, K, N, dtype, ordered)
+        got = run_linear(x, w, b, dy, groups)
+        r = (ids >= 0) & (ids < G)
+        X, W, B, D = x.double()[r], w.double()[ids[r]], b.double()[ids[r]], dy.double()[r]
+        n = torch.bincount(ids[r], minlength=G).double()
+
+        def put(shape, v, at):
+            return torch.zeros(shape, device=DEV, dtype=torch.float64).index_add_(0, at, v)
+        rows, own = r.nonzero()[:, 0], ids[r]
+        ref = {"y": put((R, N), torch.bmm(W, X[:, :, None])[:, :, 0] + B, rows), "dx": put((R, K), torch.bmm(D[:, None], W)[:, 0], rows),
+               "dw": put((G, N, K), D[:, :, None] * X[:, None], own), "db": put((G, N), D, own)}
+        mag = {"y": put((R, N), (torch.bmm(W.abs(), X.abs()[:, :, None])[:, :, 0] + B.abs()) * (K + 1), rows),
+               "dx": put((R, K), torch.bmm(D.abs()[:, None], W.abs())[:, 0] * N, rows),
+               "dw": put((G, N, K), D.abs()[:, :, None] * X.abs()[:, None], own) * n[:, None, None], "db": put((G, N), D.abs(), own) * n[:, None]}
+        for k in ref:
+            agree(got[k], ref[k], mag[k] * U, f"{k} ordered={ordered}")
+        assert not got["y"][~r].any() and not got["dx"][~r].any()
+
+
+def many_groups(R, G, K, N, dtype, ordered):
+    """More groups than group_rows sorts: the plan by hand."""
+    g = gen(901)
+    ids = torch.randint(-G // 10, G, (R,), generator=g, device=DEV)
+    ids = torch.where(ids < 0, G, ids)
+    if ordered:
+        ids = torch.sort(ids).values
+    order = torch.sort(ids, stable=True).indices.to(torch.int32)
+    offsets = torch.searchsorted(torch.sort(ids).values, torch.arange(G + 1, device=DEV)).to(torch.int32)
+    x, w, b, dy = (torch.randn(s, generator=g, device=DEV).to(dtype) for s in ((R, K), (G, N, K), (G, N), (R, N)))
+    return x, w, b, dy, RowGroups(None if ordered else order, offsets), ids
+
+
+def test_too_many_groups_are_refused():
+    G = 1 << 27
+    w, offsets = torch.zeros(1, 1, 1, device=DEV, dtype=BF16).expand(G, 1, 1), torch.zeros(G + 1, device=DEV, dtype=torch.int32)
+    with pytest.raises(ValueError, match="too many"):
+        grouped_linear(torch.zeros(1, 1, device=DEV, dtype=BF16), w, RowGroups(None, offsets))

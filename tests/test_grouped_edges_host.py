@@ -7,7 +7,7 @@ import torch
 from torch.autograd import forward_ad
 
 from grouped_checks import agree, agree_as_fp32
-from mcmc_amd import RowGroups, grouped, grouped_linear, philox_dropout
+from mcmc_amd import RowGroups, _lib, grouped, grouped_linear, philox_dropout
 
 
 @pytest.fixture
@@ -59,3 +59,16 @@ def test_the_comparison_sees_every_wrong_value(bad):
             agree(torch.ones(3), ref, tol, "a mistake of the test")
     with pytest.raises(AssertionError, match="infinities"):
         agree_as_fp32(torch.full((3,), 3e38), one * 1e39, slack, "beyond fp32")
+
+
+@pytest.mark.parametrize("product", [0, 1])
+@pytest.mark.parametrize("dtype", [_lib.DT_F32, _lib.DT_BF16, _lib.DT_F16])
+def test_walks_of_many_groups_end(product, dtype):
+    """Every workgroup of a forward or dx product walks all offsets: groups times workgroups is bounded, whatever the widths."""
+    size = _lib.load().mcmc_grouped_linear_workspace_bytes
+    for n_in, n_out in ((1, 1), (64, 64), (300, 200), (4096, 64), (64, 4096), (2048, 2048)):
+        for rows, groups in ((1 << 20, 1 << 20), (1 << 30, 1 << 20), (1, 1 << 27), (1 << 10, 1 << 30), (1 << 30, 1 << 30)):
+            assert size(product, dtype, rows, groups, n_in, n_out) == -1 and "too many" in _lib.last_error(), (rows, groups, n_in, n_out)
+            assert size(2, dtype, rows, groups, n_in, n_out) >= 0  # the weight gradient does not walk
+        for rows, groups in ((1 << 24, 63), (1 << 24, 64), (1 << 22, 512), (1 << 17, 4096), (8192, 4096), (1 << 10, 1 << 16), (0, 1 << 30)):
+            assert size(product, dtype, rows, groups, n_in, n_out) >= 0, (rows, groups, n_in, n_out)
