@@ -166,19 +166,20 @@ class _GroupedLinear(torch.autograd.Function):
             y = _forward(eng, x, weight, None if bias is None else bias.contiguous(), order, offsets)
         need_x, need_w, need_b = ctx.needs_input_grad[1:4]
         (R, K), (G, N, _), dt = x.shape, weight.shape, _DT[x.dtype]
-        ctx.eng, ctx.sizes = eng, (dt, R, G, K, N, x.stride(0))
+        K_w = K if need_w else 1  # inputs of the weight gradient: db alone comes with one column of it, see backward
+        ctx.eng, ctx.sizes, ctx.needs = eng, (dt, R, G, K, K_w, N, x.stride(0)), (need_x, need_w, need_b)
         ctx.ws = (_workspace_bytes(eng, _lib.GROUPED_GRAD_INPUT, dt, R, G, K, N) if need_x else 0,
-                  _workspace_bytes(eng, _lib.GROUPED_GRAD_WEIGHT, dt, R, G, K, N) if need_w or need_b else 0)
+                  _workspace_bytes(eng, _lib.GROUPED_GRAD_WEIGHT, dt, R, G, K_w, N) if need_w or need_b else 0)
         # what each gradient reads: dx the weights, dW the inputs
-        ctx.save_for_backward(x if need_w or need_b else None, weight if need_x else None, order, offsets)
+        ctx.save_for_backward(x if need_w else None, weight if need_x else None, order, offsets)
         return y
 
     @staticmethod
     @_once
     def backward(ctx, dy):
-        eng, (dt, R, G, K, N, ld_x), (ws_x, ws_w) = ctx.eng, ctx.sizes, ctx.ws
+        eng, (dt, R, G, K, K_w, N, ld_x), (ws_x, ws_w) = ctx.eng, ctx.sizes, ctx.ws
         x, weight, order, offsets = ctx.saved_tensors
-        _, need_x, need_w, need_b, _, _ = ctx.needs_input_grad
+        need_x, need_w, need_b = ctx.needs
         dx = dw = db = None
         with _on(eng):
             lib, handle, stream, dtype, dev = eng.lib, eng.ctx.handle, _stream(eng), dy.dtype, dy.device
@@ -193,10 +194,12 @@ class _GroupedLinear(torch.autograd.Function):
                 _lib.check(lib.mcmc_grouped_linear_grad_input(handle, dt, dy_p, ld_dy, R, order_p, offsets_p, G, K, N, weight.data_ptr(), dx.data_ptr(),
                                                               _ptr(ws), stream), "mcmc_grouped_linear_grad_input")
             if need_w or need_b:
-                dw = torch.empty((G, N, K), dtype=dtype, device=dev)
+                # db alone: dy stands for an x of one column, so that dy is read once and next to nothing else is done
+                x_p, ld_x = (x.data_ptr(), ld_x) if need_w else (dy_p, ld_dy)
+                dw = torch.empty((G, N, K_w), dtype=dtype, device=dev)
                 db = torch.empty((G, N), dtype=dtype, device=dev) if need_b else None
                 ws = _workspace(ws_w, dev)
-                _lib.check(lib.mcmc_grouped_linear_grad_weight(handle, dt, dy_p, ld_dy, x.data_ptr(), ld_x, R, order_p, offsets_p, G, K, N, dw.data_ptr(),
+                _lib.check(lib.mcmc_grouped_linear_grad_weight(handle, dt, dy_p, ld_dy, x_p, ld_x, R, order_p, offsets_p, G, K_w, N, dw.data_ptr(),
                                                                _ptr(db), _ptr(ws), stream), "mcmc_grouped_linear_grad_weight")
         return None, dx, dw if need_w else None, db, None, None
 

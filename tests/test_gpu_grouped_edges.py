@@ -248,3 +248,33 @@ def test_too_many_groups_are_refused():
     w, offsets = torch.zeros(1, 1, 1, device=DEV, dtype=BF16).expand(G, 1, 1), torch.zeros(G + 1, device=DEV, dtype=torch.int32)
     with pytest.raises(ValueError, match="too many"):
         grouped_linear(torch.zeros(1, 1, device=DEV, dtype=BF16), w, RowGroups(None, offsets))
+
+
+# ------------------------------------------------------------------------------------------------- a bias alone
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("R, G, K, N", [(1, 1, 1, 1), (37, 5, 11, 256), (100, 3, 24, 40), (60_000, 3, 64, 48), (20_000, 9, 64, 1), (9000, 1, 200, 136),
+                                        (3000, 8, 2048, 2048), (300, 600, 7, 33)])
+def test_the_gradient_of_the_bias_alone(R, G, K, N, dtype):
+    """Frozen weights: db needs neither x nor a dW, which would be G N K elements."""
+    for ordered in (False, True):
+        x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, 950, ordered, 0.1)
+        wide = torch.randn(R, N + 3, generator=gen(951), device=DEV).to(dtype)
+        b.requires_grad_()
+        y = grouped_linear(x, w, groups, b)
+        x.fill_(float("nan"))  # not read any more
+        for d in (dy, wide[:, 1:N + 1], dy[:1].expand(R, N)):
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            db, = torch.autograd.grad(y, b, d, retain_graph=True)
+            assert torch.cuda.max_memory_allocated() - before <= 64 * G * N + (1 << 22)
+            ref, mag = torch.zeros(G, N, device=DEV, dtype=torch.float64), torch.zeros(G, N, device=DEV, dtype=torch.float64)
+            own = (ids >= 0) & (ids < G)
+            ref.index_add_(0, ids[own], d.double()[own])
+            mag.index_add_(0, ids[own], d.double().abs()[own])
+            agree(db, ref, mag * torch.bincount(ids[own], minlength=G).double()[:, None] * U, "db")
+        with pytest.raises(RuntimeError):  # x is saved for dW, and was changed since
+            xs, ws = torch.zeros_like(x), w.detach().requires_grad_()
+            y = grouped_linear(xs, ws, groups, b)
+            xs.add_(1)
+            y.sum().backward()
