@@ -450,7 +450,8 @@ int mcmc_group_rows(mcmc_ctx* ctx, const void* ids, int id_bytes, int64_t rows, 
 
 /* y[r] = weight[g] x[r] + bias[g] for every row r of every group g (F.linear, bayesian_ensemble.py:49, with the group's own
  * weights); rows of no group get 0.
- *   dtype   MCMC_DT_F32, MCMC_DT_BF16 or MCMC_DT_F16: of x, weight, bias, y and all gradients; sums are fp32
+ *   dtype   MCMC_DT_F32, MCMC_DT_BF16 or MCMC_DT_F16: of x, weight, bias, y and all gradients; sums are fp32.  MCMC_DT_F32: a product is
+ *           off by up to 2^-23 of itself; operands below 2^-110 in magnitude count with an absolute error of up to 2^-134
  *   x       [rows, n_in], ld_x elements between rows (any, also 0);  y [rows, n_out] dense
  *   weight  [n_groups, n_out, n_in] dense;  bias [n_groups, n_out] or NULL
  *   order   [rows] int32, every row once, or NULL (row r is at position r);  offsets [n_groups + 1] int32, from 0, not

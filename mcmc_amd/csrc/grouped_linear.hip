@@ -81,9 +81,10 @@ struct Frag<_Float16> {
     static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 d) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, d, 0, 0, 0); }
 };
 // fp32 on the bf16 pipe: the fp32 matrix instructions run at 1/16 of its rate.  x = h + m + l with h = x rounded to bf16's 8 bits, m =
-// the rest rounded likewise, l = what is left (at most 8 bits: exact, down to 2^-126); of the nine products the six down to h l +
-// m m + l h are summed in fp32, the small ones first, so that a short sum is rounded once.  Left out: m l + l m + l l, below
-// 2^-26 |x y|, a quarter of an fp32 rounding.  Near the top of the range the six are not the product: an operand that rounds to an
+// the rest rounded likewise, l = what is left (at most 8 bits); of the nine products the six down to h l + m m + l h are summed in
+// fp32, the small ones first, so that a short sum is rounded once.  Left out: m l + l m + l l, at most 2^-24 |x y| (|m| <= 2^-8 |x|, |l| <=
+// 2^-17 |x|), one fp32 rounding.  The split is exact down to |x| = 2^-110; below, l ends at bf16's smallest number, 2^-133 (the matrix
+// instructions keep subnormals), so that x is off by up to 2^-134 however small it is.  Near the top of the range the six are not the product: an operand that rounds to an
 // infinity has no such split (inf - inf), of a product that overflows, or nearly does, some terms are infinite and of either sign.  All of
 // these end in a sum that is not finite, and infinities and NaN stay: such a sum is done over, one product after the other (plain_sums).
 template <>

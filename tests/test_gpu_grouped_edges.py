@@ -278,3 +278,63 @@ def test_the_gradient_of_the_bias_alone(R, G, K, N, dtype):
             y = grouped_linear(xs, ws, groups, b)
             xs.add_(1)
             y.sum().backward()
+
+
+# ------------------------------------------------------------------------------------------ the bottom of the range
+TINY = [(300, 3, 40, 33), (500, 3, 256, 128), (500, 3, 300, 200), (500, 2, 200, 300), (9, 2, 2048, 64), (9, 2, 64, 2048), (600, 2, 2048, 2056),
+        (60_000, 3, 64, 48), (20_000, 2, 64, 1), (20_000, 2, 11, 256)]
+
+
+@pytest.mark.parametrize("e", [-105, -112, -118, -126, -140])
+@pytest.mark.parametrize("R, G, K, N", TINY)
+def test_fp32_operands_at_the_bottom_of_the_range(R, G, K, N, e):
+    """x and dy, then the weights, about 2^e against 2^100: operands below 2^-110 are off by up to 2^-134 each, on top of a sum's usual bound."""
+    x, w, b, dy, groups, ids = linear_case(R, G, K, N, FP32, 970)
+    step = 2.0 ** -134
+    for small, large in (((x, dy), (w,)), ((w,), (x, dy))):
+        x2, w2, dy2 = (t * (2.0 ** e if any(t is s for s in small) else 2.0 ** 100) for t in (x, w, dy))
+        got = run_linear(x2, w2, b * 0, dy2, groups)
+        ref, mag = linear_reference(x2, w2, b * 0, dy2, ids)
+        _, other = linear_reference(torch.ones_like(x2), w2, b * 0, torch.ones_like(dy2), ids)  # (K + 1) sum |w|, N sum |w|
+        _, mine = linear_reference(x2, torch.ones_like(w2), b * 0, dy2, ids)                     # (K + 1) sum |x|, N sum |dy|
+        agree(got["y"], ref["y"], mag["y"] * U + step * (other["y"] + mine["y"]) / (K + 1), "y")
+        agree(got["dx"], ref["dx"], mag["dx"] * U + step * (other["dx"] + mine["dx"]) / N, "dx")
+        if small[0] is x:
+            n = torch.bincount(ids, minlength=G).double()[:, None]
+            agree(got["db"], ref["db"], mag["db"] * U + n * step, "db")
+    x2, dy2 = x * 2.0 ** e, dy * 2.0 ** 100
+    for x2, dy2 in ((x2, dy2), (x * 2.0 ** 100, dy * 2.0 ** e)):
+        got = run_linear(x2, w, b, dy2, groups)["dw"]
+        ref, mag = linear_reference(x2, w, b, dy2, ids)
+        _, a = linear_reference(x2, w, b, torch.ones_like(dy2), ids)
+        _, c = linear_reference(torch.ones_like(x2), w, b, dy2, ids)
+        n = torch.bincount(ids, minlength=G).double().clamp(min=1)[:, None, None]
+        agree(got, ref["dw"], mag["dw"] * U + step * (a["dw"] + c["dw"]) / n, "dw")
+
+
+@pytest.mark.parametrize("dtype, small, large", [(FP16, 2.0 ** -24, 2.0 ** 9), (BF16, 2.0 ** -133, 2.0 ** 40)])
+@pytest.mark.parametrize("R, G, K, N", ONE_HOT)
+def test_subnormal_operands_count(R, G, K, N, dtype, small, large):
+    """16-bit operands of one to 64 times the type's smallest number against a power of two, one product a sum: exact."""
+    x, w, b, dy, groups, ids = linear_case(R, G, K, N, dtype, 990)
+    g, rows, zero = gen(991), torch.arange(R, device=DEV), torch.zeros_like(b)
+
+    def tiny(shape):
+        return (torch.randint(1, 65, shape, generator=g, device=DEV).double() * small).to(dtype)
+    for left, right in ((tiny((R,)), torch.full((G, N, K), large, device=DEV, dtype=dtype)), (torch.full((R,), large, device=DEV, dtype=dtype), tiny((G, N, K)))):
+        xs, ds = torch.zeros_like(x), torch.zeros_like(dy)
+        xs[rows, rows % K], ds[rows, rows % N] = left, left
+        same(grouped_linear(xs, right, groups, zero), left.double()[:, None] * right.double()[ids, :, rows % K], "y")
+        same(run_linear(xs, right, zero, ds, groups)["dx"], left.double()[:, None] * right.double()[ids, rows % N], "dx")
+    xs, ds = tiny((R, K)), torch.zeros_like(dy)
+    dw, db = torch.zeros(G, N, K, device=DEV, dtype=torch.float64), torch.zeros(G, N, device=DEV, dtype=torch.float64)
+    for i in range(G):
+        of = (ids == i).nonzero()[:, 0][:N]
+        cols = torch.arange(of.numel(), device=DEV)
+        ds[of, cols] = large
+        dw[i, cols], db[i, cols] = large * xs[of].double(), large
+    got = run_linear(xs, w, b, ds, groups)
+    same(got["dw"], dw, "dw")
+    same(got["db"], db, "db")
+    ds = torch.where(ds != 0, tiny(ds.shape), torch.zeros_like(ds))
+    same(run_linear(xs, w, b, ds, groups)["db"], torch.zeros_like(db).index_add_(0, ids, ds.double()), "db")
