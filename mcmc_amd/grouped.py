@@ -167,7 +167,7 @@ class _GroupedLinear(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[1:4]
         (R, K), (G, N, _), dt = x.shape, weight.shape, _DT[x.dtype]
         K_w = K if need_w else 1  # inputs of the weight gradient: db alone comes with one column of it, see backward
-        ctx.eng, ctx.sizes, ctx.needs = eng, (dt, R, G, K, K_w, N, x.stride(0)), (need_x, need_w, need_b)
+        ctx.eng, ctx.sizes, ctx.needs = eng, (dt, R, G, K, K_w, N), (need_x, need_w, need_b)
         ctx.ws = (_workspace_bytes(eng, _lib.GROUPED_GRAD_INPUT, dt, R, G, K, N) if need_x else 0,
                   _workspace_bytes(eng, _lib.GROUPED_GRAD_WEIGHT, dt, R, G, K_w, N) if need_w or need_b else 0)
         # what each gradient reads: dx the weights, dW the inputs
@@ -177,7 +177,7 @@ class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dy):
-        eng, (dt, R, G, K, K_w, N, ld_x), (ws_x, ws_w) = ctx.eng, ctx.sizes, ctx.ws
+        eng, (dt, R, G, K, K_w, N), (ws_x, ws_w) = ctx.eng, ctx.sizes, ctx.ws
         x, weight, order, offsets = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs
         dx = dw = db = None
@@ -187,19 +187,22 @@ class _GroupedLinear(torch.autograd.Function):
             if not dy.is_contiguous():
                 dy = _rows(dy)
                 ld_dy = dy.stride(0)
+            # what was saved may come back with other strides (hooks on saved tensors)
+            order, offsets = None if order is None else order.contiguous(), offsets.contiguous()
             dy_p, order_p, offsets_p = dy.data_ptr(), _ptr(order), offsets.data_ptr()
             if need_x:
+                weight = weight.contiguous()
                 dx = torch.empty((R, K), dtype=dtype, device=dev)
                 ws = _workspace(ws_x, dev)
                 _lib.check(lib.mcmc_grouped_linear_grad_input(handle, dt, dy_p, ld_dy, R, order_p, offsets_p, G, K, N, weight.data_ptr(), dx.data_ptr(),
                                                               _ptr(ws), stream), "mcmc_grouped_linear_grad_input")
             if need_w or need_b:
                 # db alone: dy stands for an x of one column, so that dy is read once and next to nothing else is done
-                x_p, ld_x = (x.data_ptr(), ld_x) if need_w else (dy_p, ld_dy)
+                x = _rows(x) if need_w else dy
                 dw = torch.empty((G, N, K_w), dtype=dtype, device=dev)
                 db = torch.empty((G, N), dtype=dtype, device=dev) if need_b else None
                 ws = _workspace(ws_w, dev)
-                _lib.check(lib.mcmc_grouped_linear_grad_weight(handle, dt, dy_p, ld_dy, x_p, ld_x, R, order_p, offsets_p, G, K_w, N, dw.data_ptr(),
+                _lib.check(lib.mcmc_grouped_linear_grad_weight(handle, dt, dy_p, ld_dy, x.data_ptr(), x.stride(0), R, order_p, offsets_p, G, K_w, N, dw.data_ptr(),
                                                                _ptr(db), _ptr(ws), stream), "mcmc_grouped_linear_grad_weight")
         return None, dx, dw if need_w else None, db, None, None
 
@@ -269,6 +272,7 @@ class _PhiloxDropout(torch.autograd.Function):
         R, W = ctx.sizes
         with _on(eng):
             dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
+            x = None if x is None else _rows(x)  # hooks on saved tensors may have changed its strides
             ld = W
             if not dy.is_contiguous():
                 dy = _rows(_flat(dy))

@@ -338,3 +338,14 @@ def test_subnormal_operands_count(R, G, K, N, dtype, small, large):
     same(got["db"], db, "db")
     ds = torch.where(ds != 0, tiny(ds.shape), torch.zeros_like(ds))
     same(run_linear(xs, w, b, ds, groups)["db"], torch.zeros_like(db).index_add_(0, ids, ds.double()), "db")
+
+
+# ------------------------------------------------------------------------------------------------- saved tensors elsewhere
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_saved_tensors_kept_on_the_host(dtype):
+    """What the hooks bring back is dense, whatever the strides of the view that was saved."""
+    x, w, b, dy, groups, ids = linear_case(300, 4, 63, 40, dtype, 995, ld=80)
+    want, drop = run_linear(x, w, b, dy, groups), run_dropout(x, x, 0.2, 3, activation="elu")
+    with torch.autograd.graph.save_on_cpu():
+        got, again = run_linear(x, w, b, dy, groups), run_dropout(x, x, 0.2, 3, activation="elu")
+    assert all(torch.equal(got[n], want[n]) for n in want) and all(torch.equal(again[n], drop[n]) for n in drop)

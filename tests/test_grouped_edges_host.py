@@ -72,3 +72,50 @@ def test_walks_of_many_groups_end(product, dtype):
             assert size(2, dtype, rows, groups, n_in, n_out) >= 0  # the weight gradient does not walk
         for rows, groups in ((1 << 24, 63), (1 << 24, 64), (1 << 22, 512), (1 << 17, 4096), (8192, 4096), (1 << 10, 1 << 16), (0, 1 << 30)):
             assert size(product, dtype, rows, groups, n_in, n_out) >= 0, (rows, groups, n_in, n_out)
+
+
+class Recorder:
+    """A library whose calls are kept and do nothing."""
+
+    def __init__(self):
+        self.calls = {}
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls[name] = args
+            return 0
+        return call
+
+
+def dense_copy(t):
+    return torch.empty(t.shape, dtype=t.dtype).copy_(t)
+
+
+def last_dimension_first(t):
+    return t.clone() if t.dim() < 2 else t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.parametrize("unpack", [dense_copy, last_dimension_first])
+def test_backward_reads_saved_tensors_as_they_come_back(no_device, monkeypatch, unpack):
+    """Hooks on saved tensors (offloading to the host, for one) hand back other strides than were saved."""
+    eng = SimpleNamespace(lib=Recorder(), ctx=SimpleNamespace(handle=None))
+    monkeypatch.setattr(grouped, "_engine", lambda *a, **kw: eng)
+    monkeypatch.setattr(grouped, "_stream", lambda e: 0)
+    back, groups = [], RowGroups(torch.arange(4, dtype=torch.int32), torch.tensor([0, 2, 4], dtype=torch.int32))
+
+    def unpacked(t):
+        back.append(unpack(t))
+        return back[-1]
+    x = torch.randn(4, 9)[:, 1:4].requires_grad_()  # rows 9 apart
+    w, b = torch.randn(2, 5, 3, requires_grad=True), torch.randn(2, 5, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpacked):
+        y, z = grouped_linear(x, w, groups, b), philox_dropout(x, 0.1, 1, activation="elu")
+    y.backward(torch.ones_like(y))
+    z.backward(torch.ones_like(z))
+    _, _, _, _, x_p, ld_x, *_ = eng.lib.calls["mcmc_grouped_linear_grad_weight"]
+    assert ld_x == 3  # dense, whatever it was when saved
+    assert unpack is not dense_copy or x_p in [t.data_ptr() for t in back]
+    assert eng.lib.calls["mcmc_dropout_backward"][6] == 3
+    w_p = eng.lib.calls["mcmc_grouped_linear_grad_input"][10]
+    transposed = [t.data_ptr() for t in back if not t.is_contiguous()]
+    assert w_p not in transposed and x_p not in transposed and eng.lib.calls["mcmc_dropout_backward"][5] not in transposed
