@@ -85,8 +85,9 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
 
 
 def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
-    """A forward-mode tangent does not show in requires_grad, and holds whatever the grad mode."""
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    """A forward-mode tangent does not show in requires_grad, and holds whatever the grad mode.  (Outside a dual level, number -1, there are
+    none; the callers look at the level themselves, a call less.)"""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _once(backward):
@@ -95,7 +96,7 @@ def _once(backward):
     recorded = once_differentiable(backward)
 
     def run(ctx, dy):
-        if _has_tangent(dy):
+        if forward_ad._current_level >= 0 and _has_tangent(dy):
             raise NotImplementedError("the gradients of mcmc_amd's grouped operators have no forward-mode derivative (jvp)")
         return recorded(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
     return run
@@ -103,7 +104,9 @@ def _once(backward):
 
 def _wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether the call has to pass through autograd: for a gradient, or to be refused there (no operator has a jvp)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or _has_tangent(*tensors)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and _has_tangent(*tensors)
 
 
 class RowGroups(NamedTuple):
@@ -198,11 +201,16 @@ class _GroupedLinear(torch.autograd.Function):
                                                               _ptr(ws), stream), "mcmc_grouped_linear_grad_input")
             if need_w or need_b:
                 # db alone: dy stands for an x of one column, so that dy is read once and next to nothing else is done
-                x = _rows(x) if need_w else dy
+                ld_x = K
+                if not need_w:
+                    x, ld_x = dy, ld_dy
+                elif not x.is_contiguous():
+                    x = _rows(x)
+                    ld_x = x.stride(0)
                 dw = torch.empty((G, N, K_w), dtype=dtype, device=dev)
                 db = torch.empty((G, N), dtype=dtype, device=dev) if need_b else None
                 ws = _workspace(ws_w, dev)
-                _lib.check(lib.mcmc_grouped_linear_grad_weight(handle, dt, dy_p, ld_dy, x.data_ptr(), x.stride(0), R, order_p, offsets_p, G, K_w, N, dw.data_ptr(),
+                _lib.check(lib.mcmc_grouped_linear_grad_weight(handle, dt, dy_p, ld_dy, x.data_ptr(), ld_x, R, order_p, offsets_p, G, K_w, N, dw.data_ptr(),
                                                                _ptr(db), _ptr(ws), stream), "mcmc_grouped_linear_grad_weight")
         return None, dx, dw if need_w else None, db, None, None
 
