@@ -481,7 +481,8 @@ int mcmc_grouped_linear_grad_weight(mcmc_ctx* ctx, int dtype, const void* dy, in
  *   dtype      MCMC_DT_F32, MCMC_DT_BF16 or MCMC_DT_F16
  *   activation MCMC_ACT_NONE or MCMC_ACT_ELU (alpha 1)
  *   seed_dev   device uint64 read when the kernel runs (a captured hipGraph can be replayed with a new key); NULL: `seed`
- *   0 <= p_drop < 1; elem_begin a multiple of 16, elem_begin + width <= 2^32; row_begin + rows <= 2^32; 0 <= pair < 2^32
+ *   0 <= p_drop < 1 (an element is kept with probability floor((1-p_drop) 65536) / 65536: from p_drop > 1 - 2^-16 on none is);
+ *   elem_begin a multiple of 16, elem_begin + width <= 2^32; row_begin + rows <= 2^32; 0 <= pair < 2^32
  * ld_*: elements between rows.  Pointers need the alignment of their elements only. */
 #define MCMC_ACT_NONE 0
 #define MCMC_ACT_ELU 1

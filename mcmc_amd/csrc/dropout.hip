@@ -14,8 +14,8 @@
 // even, so the two lanes always meet).
 // A dropped element is +0 whatever x holds, NaN and infinities included (a select, not a product).
 //
-// Bound: memory, 2 accesses an element forward, 3 backward with an activation.  1,048,576 x 256 bf16 with ELU: forward 193 us, backward
-// 290 us, 5.6 TB/s both; 36,501 x 1,001 fp16 (rows that start anywhere): 34 us, 4.3 TB/s.
+// Bound: memory, 2 accesses an element forward, 3 backward with an activation.  1,048,576 x 256 bf16 with ELU: forward 200 us, backward
+// 295 us, 5.4 TB/s both; 36,501 x 1,001 fp16 (rows that start anywhere): 35 us, 4.2 TB/s.
 #include "common.hpp"
 #include "elu.hpp"
 #include "philox.hpp"

@@ -193,7 +193,7 @@ constexpr int kThreads = 256;
 // Measured, 16-bit, 32,768 rows, 4096 x 4096: one group 835 / 902 / 1,020 us (forward, dx, dW: 1,317 / 1,219 / 1,078 TFLOP/s), where the
 // clock falls to what the power allows; eight groups of random sizes 1,001 / 1,030 / 1,065 (136 row tiles for 128: nine rounds of
 // workgroups for eight).  8,192 rows, 8 groups, 2048 x 2048: 97 / 105 / 82 us, 707 / 656 / 834 TFLOP/s; rows that are not whole 16-byte
-// pieces (2047 x 2045) 214 / 180 / 160.  fp32 there: 472 / 469 / 422 us, 146 / 147 / 163 TFLOP/s (the fp32 matrix instructions' dense
+// pieces (2047 x 2045) 212 / 180 / 160.  fp32 there: 454 / 458 / 415 us, 151 / 150 / 166 TFLOP/s (the fp32 matrix instructions' dense
 // product reaches 153 on this card).
 __device__ const uint4 kZeros[2] = {};
 constexpr int kSegment = 1024;  // dW: row numbers in LDS, two segments, the next one loaded while one is used
@@ -856,8 +856,10 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
 // A lane's results are four columns (m = 4 kg .. 4 kg + 3) of each of a 64-column block's four fragments.  fp32: fragment j holds columns
 // 16 j + m.  16-bit: fragments 2 h and 2 h + 1 hold columns 32 h + 8 (m >> 2) + 4 (j & 1) + (m & 3), so that two of them are eight
 // consecutive columns.  Either way a lane stores 16 bytes at a time and the four lanes of a row 64 consecutive bytes.
-// Measured, bf16, 8 groups, forward / dx (the tile kernel): 3,650,000 rows 256 -> 128 611 / 643 us (668 / 787), 4.6 / 4.4 TB/s; 1,048,576
-// rows 128 -> 64 97 / 103 (130 / 121), 64 -> 1 41 / 36 (94 / 77), 11 -> 256 161 / 152 (200 / 201).
+// Measured, bf16, 8 groups, rows gathered by `order`, one product repeated, forward / dx (the tile kernel): 3,650,000 rows 256 -> 128 657 /
+// 658 us (735 / 804), 4.3 TB/s; 1,048,576 rows 128 -> 64 93 / 102 (134 / 120), 64 -> 1 39 / 34 (95 / 77), 11 -> 256 158 / 150 (200 / 197).  Rows in
+// order: 64 -> 1 32 / 30, the others 0 to 10 % less.  The 134 MB of 64 columns stay in the last-level cache between such calls; within a training
+// step 64 -> 1 takes 43 / 37.
 constexpr int kStripWaves = 8;
 // LDS for a workgroup's weights: two workgroups a CU; fp32, whose registers allow one, most of it
 template <typename T>
@@ -999,7 +1001,8 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
 // whole accesses (16 lanes read a row's 128 columns side by side), and instruction j takes column 8 fr + j of them, so nothing is
 // turned through LDS.  16-bit: 16 rows an instruction, four rows' halves brought together; fp32: the fp32 instruction, 4 rows.
 // Four waves take turns at 64 rows of a run and meet in LDS in their order.  1,048,576 rows, 8 groups, bf16, with the chunks' sum
-// (the tile kernel): 64 -> 1 49 us (189), 2.8 TB/s; 64 -> 16 51 (64); 11 -> 256 128 (206), 4.4 TB/s.
+// (the tile kernel), rows gathered by `order`: 64 -> 1 48 us (188), 2.8 TB/s, within a training step 50 and 5 for the sum; 64 -> 16 50 (67);
+// 11 -> 256 126 (203), 4.4 TB/s.  Rows in order: 45, 46, 115.
 // THIN_OUT: thin = dy (n_out columns), db is its column sum; otherwise thin = x (n_in <= 15), and db comes from a column of ones.
 template <typename T>
 struct ThinFrag;
@@ -1223,8 +1226,8 @@ int launch_product(const Args& a, Shape sh, bool dma, unsigned blocks, hipStream
 }
 
 // The strip kernel for contractions of up to 256 elements whose weights fit the workgroups' LDS: all of them, or, where the contraction
-// is so short (64) that reading P again for every q_tile columns costs little beside the output, any number (256 -> 128 fp32, two
-// tiles: 330 us, the tile kernel 261).
+// is so short (64) that reading P again for every q_tile columns costs little beside the output, any number (524,288 rows 256 -> 128 fp32,
+// two tiles: 353 us, the tile kernel 308).
 // Returns 0 where the tile kernel is to run.
 template <typename T>
 int strip_q_tile(int n_c, int n_q) {
@@ -1248,8 +1251,8 @@ struct Strip {
     int64_t blocks;
 };
 // Rows per workgroup, whole turns of its waves: eight times the bytes of its weights in LDS and 4 KB, for what it costs to start (a workgroup
-// with fewer rows spends its time there, one with more leaves a long tail: 1,048,576 rows 11 -> 256 bf16: 1,024 rows 205 us, 256 rows 161; 256 -> 11
-// fp32: 200 and 264), but no fewer workgroups than 1,024 as long as each has a turn.
+// with fewer rows spends its time there, one with more leaves a long tail: 1,048,576 rows 11 -> 256 bf16, rule 256: 1,024 rows 203 us, 256 rows 166;
+// 256 -> 11 fp32, rule 640: 128 rows 481, 256 rows 402, 640 rows 335, 1,024 rows 351), but no fewer workgroups than 1,024 as long as each has a turn.
 template <typename T>
 Strip strip_of(int64_t rows, int G, int n_c, int n_q, int q_tile) {
     const int nc = n_c <= 32 ? 1 : n_c <= 64 ? 2 : n_c <= 128 ? 4 : 8;
