@@ -86,7 +86,7 @@ struct Frag<_Float16> {
 // 2^-17 |x|), one fp32 rounding.  The split is exact down to |x| = 2^-110; below, l ends at bf16's smallest number, 2^-133 (the matrix
 // instructions keep subnormals), so that x is off by up to 2^-134 however small it is.  Near the top of the range the six are not the product: an operand that rounds to an
 // infinity has no such split (inf - inf), of a product that overflows, or nearly does, some terms are infinite and of either sign.  All of
-// these end in a sum that is not finite, and infinities and NaN stay: such a sum is done over, one product after the other (plain_sums).
+// these end in a sum that is not finite, and infinities and NaN stay: such a sum is done over in fp32 (plain_sums).
 template <>
 struct Frag<float> {
     typedef __bf16 E;
@@ -306,24 +306,41 @@ __device__ __forceinline__ void store_some(T* row, int q, int width, Value value
     }
 }
 
-// s[k] += p(c) q(c, k) for c = 0 .. n - 1, one fp32 product after the other; only those of the bits `which` count, and once they are all NaN
-// they stay so.  Slow, and rare; its registers must not crowd the products before it, hence one element of the contraction at a time.
-template <int N, typename P, typename Q>
-__device__ __forceinline__ void plain_sums(int n, unsigned which, float (&s)[N], P p, Q q) {
-    static_assert(N <= 32, "");
-    for (int c0 = 0; c0 < n; c0 += 8) {
+// fp32: of the 16 x 16 N results of N fragments, those that are not finite (see Frag<float>) once more, from memory, with the fp32 matrix
+// instructions, which follow fp32's rules.  p(c): element c of the contraction for row l & 15 of P, q(c, j): for column l & 15 of Q's fragment
+// j; lane l asks for c = l >> 4, + 4, + 8 ...; start(j, e): what result e of fragment j starts from.  All lanes of a wave take part or none.
+// Rare, so it is short rather than fast; what is NaN stays so, and once all of them are, it ends.  32,768 rows, 8 groups, 2048 x 2048, one row of
+// infinities: dW 5 ms more (its sums all have that row), forward and NaN no more than without; all infinities: 23 ms more.
+template <int N, typename Start, typename P, typename Q>
+__device__ __forceinline__ void plain_sums(f32x4 (&acc)[N], bool valid, Start start, int n, P p, Q q) {
+    static_assert(N <= 8, "");
+    float all = 0.0f;  // not finite if one of them is not
+#pragma unroll
+    for (int k = 0; k < 4 * N; ++k) all += acc[k >> 2][k & 3];
+    if (!__any(valid && !__builtin_isfinite(all))) return;
+    unsigned which = 0;
+    f32x4 s[N];
+#pragma unroll
+    for (int k = 0; k < 4 * N; ++k) {
+        which |= (unsigned)(valid && !__builtin_isfinite(acc[k >> 2][k & 3])) << k;
+        s[k >> 2][k & 3] = start(k >> 2, k & 3);
+    }
+    const int kg = (threadIdx.x & 63) >> 4;
+    for (int c0 = 0; c0 < n; c0 += 16) {
         bool open = false;
 #pragma unroll
-        for (int k = 0; k < N; ++k) open |= (which >> k & 1) && !__builtin_isnan(s[k]);
-        if (!open) return;
-#pragma unroll 1
-        for (int c = c0; c < n && c < c0 + 8; ++c) {
-            const float x = p(c);
+        for (int k = 0; k < 4 * N; ++k) open |= (which >> k & 1) && !__builtin_isnan(s[k >> 2][k & 3]);
+        if (!__any(open)) break;
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (which >> k & 1) s[k] = fmaf(x, q(c, k), s[k]);
+        for (int d = 0; d < 16; d += 4) {
+            const int c = c0 + d + kg;
+            const float x = c < n ? p(c) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(c < n ? q(c, j) : 0.0f, x, s[j], 0, 0, 0);
         }
     }
+#pragma unroll
+    for (int k = 0; k < 4 * N; ++k) acc[k >> 2][k & 3] = which >> k & 1 ? s[k >> 2][k & 3] : acc[k >> 2][k & 3];
 }
 
 // workgroup id -> tile id: ids go round the eight XCDs, each XCD gets a contiguous run of tiles (its L2 sees neighbours)
@@ -748,23 +765,21 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
         const int r = a.order ? a.order[tl.first + c] : tl.first + c;
         return (unsigned)r < (unsigned)rows ? (float)base[(int64_t)r * ld + col] : 0.0f;
     };
-    uint64_t again = 0;  // fp32: this lane's sums that are not finite (see Frag<float>), bit (i FQ + j) 4 + e
     if constexpr (kWide) {
-        static_assert(FP * FQ * 4 <= 64 && FQ * 4 <= 16, "a bit for every sum");
-        float all = 0.0f;  // not finite if one of them is not
 #pragma unroll
-        for (int i = 0; i < FP; ++i)
-#pragma unroll
-            for (int j = 0; j < FQ; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) all += acc[i][j][e];
-        if (!__builtin_isfinite(all))
-#pragma unroll
-            for (int i = 0; i < FP; ++i)
-#pragma unroll
-                for (int j = 0; j < FQ; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) again |= (uint64_t)!__builtin_isfinite(acc[i][j][e]) << ((i * FQ + j) * 4 + e);
+        for (int i = 0; i < FP; ++i) {
+            const int p = pw + 16 * i + fr, row = kPCols ? p0 + p : rows_lds[p];
+            const bool valid = kPCols ? row < n_p : row >= 0;
+            plain_sums(
+                acc[i], valid, [](int, int) { return 0.0f; }, n_c,
+                [&](int c) { return !valid ? 0.0f : kPCols ? plain_element(P, a.ld_p, c, row) : (float)P[(int64_t)row * a.ld_p + c]; },
+                [&](int c, int j) {
+                    const int q = q0 + qw + 16 * j + fr;
+                    if (q >= n_q) return 0.0f;
+                    return PRODUCT == kGradWeight ? plain_element(Q, a.ld_q, c, q)
+                                                  : (float)Q[PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)c * a.ld_q + q];
+                });
+        }
     }
 
     // ---- lane: output row fr of P's fragment i, and of Q's fragments the columns column(j) .. + 3 (paired: of two, eight)
@@ -808,41 +823,16 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void grouped_tile_kernel(Args a) {
             float v = sumb[i] + accb[i];  // of the rows 8 kg .. 8 kg + 7 of every 32
             v += __shfl_xor(v, 16);
             v += __shfl_xor(v, 32);
-            if (kg != 0) continue;
-            if (kWide && !__builtin_isfinite(v)) {
-                float s[1] = {};
-                plain_sums(n_c, 1, s, [&](int c) { return plain_element(P, a.ld_p, c, p0 + p); }, [](int, int) { return 1.0f; });
-                v = s[0];
+            if (kWide && !__builtin_isfinite(v)) {  // (the four lanes of a column agree)
+                v = 0.0f;
+#pragma unroll 8
+                for (int c = kg; c < n_c; c += 4) v += plain_element(P, a.ld_p, c, p0 + p);
+                v += __shfl_xor(v, 16);
+                v += __shfl_xor(v, 32);
             }
+            if (kg != 0) continue;
             if (a.chunk_rows) a.part[(int64_t)a.chunks * a.n_out * a.n_in + (int64_t)run * a.n_out + p0 + p] = v;
             else static_cast<T*>(a.dbias)[(int64_t)tl.g * a.n_out + p0 + p] = (T)v;
-        }
-    }
-    if constexpr (kWide) {
-        constexpr unsigned kRow = (1u << (FQ * 4)) - 1;
-        for (int i = 0; again; ++i, again >>= FQ * 4) {
-            const int p = pw + 16 * i + fr, row = kPCols ? p0 + p : rows_lds[p];
-            unsigned which = (unsigned)again & kRow;
-#pragma unroll
-            for (int k = 0; k < FQ * 4; ++k)
-                if (column(k >> 2) + (k & 3) >= n_q) which &= ~(1u << k);
-            if (!which || (kPCols ? row >= n_p : row < 0)) continue;
-            float s[FQ * 4] = {};
-            plain_sums(
-                n_c, which, s, [&](int c) { return kPCols ? plain_element(P, a.ld_p, c, row) : (float)P[(int64_t)row * a.ld_p + c]; },
-                [&](int c, int k) {
-                    const int q = column(k >> 2) + (k & 3);
-                    return PRODUCT == kGradWeight ? plain_element(Q, a.ld_q, c, q)
-                                                  : (float)Q[PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)c * a.ld_q + q];
-                });
-            float* const out = PRODUCT == kGradWeight ? (a.chunk_rows ? a.part : static_cast<float*>(a.out)) + ((int64_t)run * a.n_out + row) * a.n_in
-                               : a.splits > 1         ? a.part + ((int64_t)split * rows + row) * n_q
-                                                      : static_cast<float*>(a.out) + (int64_t)row * n_q;
-#pragma unroll
-            for (int k = 0; k < FQ * 4; ++k) {
-                const int q = column(k >> 2) + (k & 3);
-                if (which >> k & 1) out[q] = s[k] + (bias ? (float)bias[q] : 0.0f);
-            }
         }
     }
 }
@@ -969,28 +959,19 @@ __global__ __launch_bounds__(64 * kStripWaves, sizeof(T) == 4 ? 2 : 4) void grou
                         for (int j = 0; j < 4; ++j) acc[j] = F::mfma(*reinterpret_cast<const V*>(w + m * plane_bytes + (j * NC + k) * 1024), q[l], acc[j]);
                 if (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);  // (all k's splits and reads at once would not fit the registers)
             }
+            if constexpr (sizeof(T) == 4)
+                plain_sums(
+                    acc, out_row >= 0 && !none, [&](int j, int e) { return bias[column(b, j) + e]; }, n_c,
+                    [&](int c) { return out_row < 0 ? 0.0f : (float)P[(int64_t)out_row * a.ld_p + c]; },
+                    [&](int c, int j) {
+                        const int q = q0 + 64 * b + 16 * j + fr;
+                        if (q >= n_q) return 0.0f;
+                        return (float)W[PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)c * a.ld_q + q];
+                    });
             if (out_row < 0) continue;
             constexpr int kOnce = 16 / sizeof(T);
 #pragma unroll
             for (int j = 0; j < 4; j += kOnce / 4) store_some<T, kOnce>(out, column(b, j), width, [&](int e) { return acc[j + (e >> 2)][e & 3]; });
-            if constexpr (sizeof(T) == 4) {  // sums that are not finite (see Frag<float>)
-                float all = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 16; ++k) all += acc[k >> 2][k & 3];
-                if (__builtin_isfinite(all) || none) continue;
-                unsigned again = 0;
-#pragma unroll
-                for (int k = 0; k < 16; ++k) again |= (unsigned)!__builtin_isfinite(acc[k >> 2][k & 3]) << k;
-                for (; again; again &= again - 1) {
-                    const int k = __ffs(again) - 1, in = column(b, k >> 2) + (k & 3), q = q0 + in;
-                    if (in >= width) continue;
-                    float s[1] = {bias[in]};
-                    plain_sums(
-                        n_c, 1, s, [&](int c) { return (float)P[(int64_t)out_row * a.ld_p + c]; },
-                        [&](int c, int) { return (float)W[PRODUCT == kForward ? (int64_t)q * a.ld_q + c : (int64_t)c * a.ld_q + q]; });
-                    out[in] = s[0];
-                }
-            }
         }
     }
 }
