@@ -310,7 +310,7 @@ __device__ __forceinline__ void store_some(T* row, int q, int width, Value value
 // instructions, which follow fp32's rules.  p(c): element c of the contraction for row l & 15 of P, q(c, j): for column l & 15 of Q's fragment
 // j; lane l asks for c = l >> 4, + 4, + 8 ...; start(j, e): what result e of fragment j starts from.  All lanes of a wave take part or none.
 // Rare, so it is short rather than fast; what is NaN stays so, and once all of them are, it ends.  32,768 rows, 8 groups, 2048 x 2048, one row of
-// infinities: dW 5 ms more (its sums all have that row), forward and NaN no more than without; all infinities: 23 ms more.
+// infinities: the gradient pass 6 ms more (all of dW has that row), forward and NaN no more than without; all infinities: 27 ms more.
 template <int N, typename Start, typename P, typename Q>
 __device__ __forceinline__ void plain_sums(f32x4 (&acc)[N], bool valid, Start start, int n, P p, Q q) {
     static_assert(N <= 8, "");

@@ -303,8 +303,9 @@ def philox_dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], *,
 
     activation: None or "elu" (alpha 1), applied before the dropout.  p in [0, 1), taken in float32; the keep probability is
     (1 - p) rounded down to a multiple of 2^-16 while the scale stays 1 / (1 - p), as in the fused kernels: the mean is low by up to
-    2^-16 / (1 - p) of itself (1.5e-4 at p = 0.9), and from p > 1 - 2^-16 on everything is dropped.  seed: a 64-bit integer, or a one-element int64 tensor on x's device that is read when the kernel
-    runs, so that a captured graph can be replayed with other masks (keep its value until the backward pass has run)."""
+    2^-16 / (1 - p) of itself (1.5e-4 at p = 0.9), and from p > 1 - 2^-16 on everything is dropped.  seed: a 64-bit integer, or a
+    one-element int64 tensor on x's device that is read when the kernel runs, so that a captured graph can be replayed with other
+    masks (keep its value until the backward pass has run)."""
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
     _dtype(x, "x")
